@@ -1,5 +1,6 @@
-"""In-tree build of libfarq.so and libdsa_topk.so (the sm_100a kernels behind
-the C ABIs in include/farq.h and include/dsa_topk.h).
+"""In-tree build of libfarq.so, libdsa_topk.so and libdsa_kv.so (the sm_100a
+kernels behind the C ABIs in include/farq.h, include/dsa_topk.h and
+include/dsa_kv.h).
 
 The library is compiled with nvcc directly (no torch headers): it exports only
 plain-C entry points, so the Python host binds it with ctypes. The built file
@@ -24,6 +25,10 @@ LIB_PATH = PKG_DIR / "libfarq.so"
 TOPK_SOURCES = [CSRC_DIR / "dsa_topk.cu"]
 TOPK_HEADERS = [INCLUDE_DIR / "dsa_topk.h", CSRC_DIR / "dsa_topk_kernel.cuh"]
 TOPK_LIB_PATH = PKG_DIR / "libdsa_topk.so"
+
+KV_SOURCES = sorted(CSRC_DIR.glob("dsa_kv*.cu"))
+KV_HEADERS = [INCLUDE_DIR / "dsa_kv.h", *sorted(CSRC_DIR.glob("kv_*.cuh"))]
+KV_LIB_PATH = PKG_DIR / "libdsa_kv.so"
 
 OBJ_DIR = PKG_DIR / "_build"
 
@@ -54,6 +59,10 @@ def is_topk_stale() -> bool:
     return _stale(TOPK_LIB_PATH, TOPK_SOURCES + TOPK_HEADERS)
 
 
+def is_kv_stale() -> bool:
+    return _stale(KV_LIB_PATH, KV_SOURCES + KV_HEADERS)
+
+
 def _run(cmd: list[str], verbose: bool) -> str:
     if verbose:
         print(" ".join(cmd))
@@ -75,6 +84,13 @@ def build_topk_lib(force: bool = False, verbose: bool = False) -> Path:
     if not force and not is_topk_stale():
         return TOPK_LIB_PATH
     return _compile(TOPK_SOURCES, TOPK_LIB_PATH, verbose)
+
+
+def build_kv_lib(force: bool = False, verbose: bool = False) -> Path:
+    """Compile libdsa_kv.so for sm_100a if it is missing or older than its sources."""
+    if not force and not is_kv_stale():
+        return KV_LIB_PATH
+    return _compile(KV_SOURCES, KV_LIB_PATH, verbose)
 
 
 FAST_SOURCE = CSRC_DIR / "farq_fast.cpp"
@@ -116,7 +132,8 @@ def build_fast_ext(force: bool = False, verbose: bool = False) -> Path:
 
 
 def build_all(force: bool = False, verbose: bool = False) -> list[Path]:
-    libs = [build_lib(force, verbose), build_topk_lib(force, verbose)]
+    libs = [build_lib(force, verbose), build_topk_lib(force, verbose),
+            build_kv_lib(force, verbose)]
     return libs + [build_fast_ext(force, verbose)]
 
 

@@ -1,0 +1,249 @@
+// dsa_kv.cu — host side of libdsa_kv.so: argument validation, launch planning
+// and the C ABI declared in include/dsa_kv.h. Device code: kv_rope_kernel.cuh,
+// kv_copy_kernel.cuh.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "dsa_kv.h"
+#include "kv_copy_kernel.cuh"
+#include "kv_rope_kernel.cuh"
+
+namespace kv {
+
+bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+int index_size(int dt) { return dt == DSA_KV_INT32 ? 4 : dt == DSA_KV_INT64 ? 8 : 0; }
+bool is_16bit(int dt) { return dt == DSA_KV_BF16 || dt == DSA_KV_FP16; }
+
+constexpr int64_t kMaxIndex = 0x7fffffff;  // 32-bit indices on the device
+
+// 0 <= a * b * c < 2^31 for sizes that are not negative.
+bool fits(int64_t a, int64_t b, int64_t c) {
+  if (a == 0 || b == 0 || c == 0) return true;
+  if (a > kMaxIndex || b > kMaxIndex || c > kMaxIndex) return false;
+  return (double)a * (double)b * (double)c <= (double)kMaxIndex;
+}
+
+// Strides of a dense tensor: a multiple of 8 elements wherever they are used,
+// and rows of an output that do not lie on one another by a stride of 0.
+int check_dense(const dsa_kv_dense_t& t, int64_t B, int64_t Q, int64_t H, bool output) {
+  if (!t.ptr) return DSA_KV_ERR_NULL_POINTER;
+  if (!aligned(t.ptr, 16)) return DSA_KV_ERR_ALIGNMENT;
+  const int64_t n[3] = {B, Q, H}, s[3] = {t.stride_b, t.stride_q, t.stride_h};
+  for (int i = 0; i < 3; ++i) {
+    if (n[i] <= 1) continue;
+    if (s[i] % 8 != 0) return DSA_KV_ERR_ALIGNMENT;
+    if (s[i] < 0 || (output && s[i] == 0)) return DSA_KV_ERR_BAD_SHAPE;
+  }
+  return DSA_KV_OK;
+}
+Dense dense(const dsa_kv_dense_t& t) {
+  Dense d;
+  d.ptr = static_cast<uint8_t*>(t.ptr);
+  d.sb = t.stride_b * 2;
+  d.sq = t.stride_q * 2;
+  d.sh = t.stride_h * 2;
+  return d;
+}
+
+int check_cache(const dsa_kv_cache_t& c, bool written) {
+  if (c.reserved0 != 0) return DSA_KV_ERR_BAD_ARGS_SIZE;
+  if (c.code_dtype != DSA_KV_INT8 && c.code_dtype != DSA_KV_E4M3) return DSA_KV_ERR_BAD_DTYPE;
+  if (c.P < 0 || c.H < 1 || c.block_size < 1) return DSA_KV_ERR_BAD_SHAPE;
+  if (c.D < 16 || c.D > 256 || c.D % 16 != 0) return DSA_KV_ERR_BAD_HEAD_DIM;
+  if (c.P > kMaxIndex || c.H > kMaxIndex || c.block_size > kMaxIndex) return DSA_KV_ERR_UNSUPPORTED;
+  if (c.P == 0) return DSA_KV_OK;  // no page is ever followed
+  if (!c.k_codes || !c.v_codes || !c.k_scale || !c.v_scale) return DSA_KV_ERR_NULL_POINTER;
+  if (!aligned(c.k_codes, 16) || !aligned(c.v_codes, 16) || !aligned(c.k_scale, 4) || !aligned(c.v_scale, 4))
+    return DSA_KV_ERR_ALIGNMENT;
+  const int64_t n[3] = {c.P, c.H, c.block_size};
+  for (int i = 0; i < 3; ++i) {
+    if (n[i] <= 1) continue;
+    if (c.k_stride[i] % 16 != 0 || c.v_stride[i] % 16 != 0) return DSA_KV_ERR_ALIGNMENT;
+    const int64_t least = written ? 1 : 0;
+    if (c.k_stride[i] < least || c.v_stride[i] < least || c.k_scale_stride[i] < least ||
+        c.v_scale_stride[i] < least)
+      return DSA_KV_ERR_BAD_SHAPE;
+  }
+  return DSA_KV_OK;
+}
+CacheSide side(void* codes, float* scale, const int64_t s[3], const int64_t ss[3]) {
+  CacheSide c;
+  c.codes = static_cast<uint8_t*>(codes);
+  c.scale = scale;
+  c.sp = s[0]; c.sh = s[1]; c.st = s[2];
+  c.ssp = ss[0]; c.ssh = ss[1]; c.sst = ss[2];
+  return c;
+}
+
+// Launch with programmatic stream serialisation: the kernel waits for the
+// previous one (griddepcontrol.wait) before its first global access.
+template <typename... A, typename... B>
+int launch(void (*fn)(A...), int64_t grid, int threads, size_t smem, void* stream, const B&... args) {
+  if (grid > kMaxIndex) return DSA_KV_ERR_UNSUPPORTED;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, fn, args...) == cudaSuccess ? DSA_KV_OK : DSA_KV_ERR_CUDA;
+}
+
+int lanes_of(int64_t D) { return D <= 64 ? 8 : D <= 128 ? 16 : 32; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+constexpr int kUnroll = 1;  // heads or vectors that a group of lanes holds at a time
+
+using RopeFn = void (*)(const RopeParams);
+template <typename T, bool I>
+RopeFn rope_fn(int lanes) {
+  return lanes == 8 ? rope_kernel<T, 8, kUnroll, I>
+                    : lanes == 16 ? rope_kernel<T, 16, kUnroll, I> : rope_kernel<T, 32, kUnroll, I>;
+}
+
+using CopyFn = void (*)(const CopyParams);
+template <typename T, bool E>
+CopyFn copy_fn(int lanes, bool write) {
+  if (write)
+    return lanes == 8 ? write_kernel<T, 8, kUnroll, E>
+                      : lanes == 16 ? write_kernel<T, 16, kUnroll, E> : write_kernel<T, 32, kUnroll, E>;
+  return lanes == 8 ? read_kernel<T, 8, kUnroll, E>
+                    : lanes == 16 ? read_kernel<T, 16, kUnroll, E> : read_kernel<T, 32, kUnroll, E>;
+}
+
+int rope(const dsa_kv_rope_args_t* a, void* stream) {
+  if (!a) return DSA_KV_ERR_NULL_POINTER;
+  if (a->struct_size != sizeof(*a)) return DSA_KV_ERR_BAD_ARGS_SIZE;
+  const int ib = index_size(a->pos_dtype);
+  if (!is_16bit(a->dtype) || !ib || !(is_16bit(a->gamma_dtype) || a->gamma_dtype == DSA_KV_FP32))
+    return DSA_KV_ERR_BAD_DTYPE;
+  if (a->B < 0 || a->Q < 0 || a->Hq < 0 || a->Hk < 0 || a->max_pos < 0 || (a->interleaved & ~1))
+    return DSA_KV_ERR_BAD_SHAPE;
+  if (a->D < 8 || a->D > 256 || a->D % 8 != 0 || a->rot < 0 || a->rot > a->D ||
+      a->rot % (a->interleaved ? 8 : 16) != 0)
+    return DSA_KV_ERR_BAD_HEAD_DIM;
+  if (!fits(a->B, a->Q, a->Hq) || !fits(a->B, a->Q, a->Hk) || !fits(a->B, a->Q, a->Hq + a->Hk))
+    return DSA_KV_ERR_UNSUPPORTED;
+  if (a->B == 0 || a->Q == 0 || a->Hq + a->Hk == 0) return DSA_KV_OK;
+  int st;
+  if (a->Hq > 0) {
+    if ((st = check_dense(a->q, a->B, a->Q, a->Hq, false)) != DSA_KV_OK) return st;
+    if ((st = check_dense(a->q_out, a->B, a->Q, a->Hq, true)) != DSA_KV_OK) return st;
+  }
+  if (a->Hk > 0) {
+    if ((st = check_dense(a->k, a->B, a->Q, a->Hk, false)) != DSA_KV_OK) return st;
+    if ((st = check_dense(a->k_out, a->B, a->Q, a->Hk, true)) != DSA_KV_OK) return st;
+  }
+  if ((a->Hq > 0 && !a->q_gamma) || (a->Hk > 0 && !a->k_gamma) || !a->positions ||
+      (a->rot > 0 && a->max_pos > 0 && !a->cos_sin))
+    return DSA_KV_ERR_NULL_POINTER;
+  if (!aligned(a->q_gamma, 16) || !aligned(a->k_gamma, 16) || !aligned(a->cos_sin, 16) ||
+      !aligned(a->positions, ib))
+    return DSA_KV_ERR_ALIGNMENT;
+
+  const int lanes = lanes_of(a->D), strip = 32 / lanes * kUnroll;
+  const int64_t sq = ceil_div(a->Hq, strip), strips = sq + ceil_div(a->Hk, strip);
+  RopeParams p;
+  p.q = dense(a->q);
+  p.k = dense(a->k);
+  p.q_out = dense(a->q_out);
+  p.k_out = dense(a->k_out);
+  p.q_gamma = a->q_gamma;
+  p.k_gamma = a->k_gamma;
+  p.cos_sin = a->cos_sin;
+  p.positions = a->positions;
+  p.max_pos = a->max_pos;
+  p.tasks = (uint32_t)(a->B * a->Q * strips);
+  p.strips.init((uint32_t)strips);
+  p.Q.init((uint32_t)a->Q);
+  p.strips_q = (uint32_t)sq;
+  p.Hq = (uint32_t)a->Hq;
+  p.Hk = (uint32_t)a->Hk;
+  p.D = (int32_t)a->D;
+  p.rot = (int32_t)a->rot;
+  p.gamma_dtype = a->gamma_dtype;
+  p.pos_bytes = ib;
+  p.eps = a->eps;
+  p.inv_d = 1.0f / (float)a->D;
+  const RopeFn fn = a->dtype == DSA_KV_BF16
+                        ? (a->interleaved ? rope_fn<__nv_bfloat16, true>(lanes) : rope_fn<__nv_bfloat16, false>(lanes))
+                        : (a->interleaved ? rope_fn<__half, true>(lanes) : rope_fn<__half, false>(lanes));
+  return launch(fn, ceil_div(p.tasks, kCtaWarps), kCtaThreads, 0, stream, p);
+}
+
+int copy(const dsa_kv_copy_args_t* a, void* stream, bool write) {
+  if (!a) return DSA_KV_ERR_NULL_POINTER;
+  if (a->struct_size != sizeof(*a)) return DSA_KV_ERR_BAD_ARGS_SIZE;
+  const int ib = index_size(a->pos_dtype), pb = index_size(a->page_dtype);
+  if (!is_16bit(a->dtype) || !ib || !pb) return DSA_KV_ERR_BAD_DTYPE;
+  if (a->B < 0 || a->Q < 0 || a->NB < 0) return DSA_KV_ERR_BAD_SHAPE;
+  int st = check_cache(a->cache, write);
+  if (st != DSA_KV_OK) return st;
+  const dsa_kv_cache_t& c = a->cache;
+  if (!fits(a->B, a->Q, 2 * c.H) || a->NB > kMaxIndex) return DSA_KV_ERR_UNSUPPORTED;
+  if (a->B == 0 || a->Q == 0 || a->NB == 0 || (write && c.P == 0)) return DSA_KV_OK;
+  if ((st = check_dense(a->k, a->B, a->Q, c.H, !write)) != DSA_KV_OK) return st;
+  if ((st = check_dense(a->v, a->B, a->Q, c.H, !write)) != DSA_KV_OK) return st;
+  if (!a->page_table || !a->pos) return DSA_KV_ERR_NULL_POINTER;
+  if (!aligned(a->page_table, pb) || !aligned(a->pos, ib)) return DSA_KV_ERR_ALIGNMENT;
+
+  const int lanes = lanes_of(c.D);
+  CopyParams p;
+  p.k = dense(a->k);
+  p.v = dense(a->v);
+  p.kc = side(c.k_codes, c.k_scale, c.k_stride, c.k_scale_stride);
+  p.vc = side(c.v_codes, c.v_scale, c.v_stride, c.v_scale_stride);
+  p.page_table = a->page_table;
+  p.pos = a->pos;
+  p.P = c.P;
+  p.n = (uint32_t)(a->B * a->Q * 2 * c.H);
+  p.H2.init((uint32_t)(2 * c.H));
+  p.H.init((uint32_t)c.H);
+  p.Q.init((uint32_t)a->Q);
+  p.bs.init((uint32_t)c.block_size);
+  p.NB = a->NB;
+  p.D = (int32_t)c.D;
+  p.page_bytes = pb;
+  p.pos_bytes = ib;
+  const bool e = c.code_dtype == DSA_KV_E4M3;
+  const CopyFn fn = a->dtype == DSA_KV_BF16
+                        ? (e ? copy_fn<__nv_bfloat16, true>(lanes, write) : copy_fn<__nv_bfloat16, false>(lanes, write))
+                        : (e ? copy_fn<__half, true>(lanes, write) : copy_fn<__half, false>(lanes, write));
+  const int64_t per_cta = (int64_t)kCtaWarps * (32 / lanes) * kUnroll;
+  return launch(fn, ceil_div(p.n, per_cta), kCtaThreads, 0, stream, p);
+}
+
+}  // namespace kv
+
+extern "C" {
+
+int dsa_kv_abi_version(void) { return DSA_KV_ABI_VERSION; }
+
+const char* dsa_kv_strerror(int status) {
+  switch (status) {
+    case DSA_KV_OK: return "ok";
+    case DSA_KV_ERR_NULL_POINTER: return "a required pointer is NULL";
+    case DSA_KV_ERR_BAD_SHAPE: return "bad shape: a size or a stride below its least value";
+    case DSA_KV_ERR_BAD_HEAD_DIM:
+      return "head size or rotated part not supported (rotation: D <= 256, D % 8 == 0, rot <= D, rot % 16 == 0, "
+             "interleaved rot % 8 == 0; cache: D <= 256, D % 16 == 0; attention: D 64, 128 or 256, block_size >= 8)";
+    case DSA_KV_ERR_BAD_DTYPE:
+      return "unsupported dtype (dense bf16/fp16, codes int8/e4m3, indices int32/int64, gamma bf16/fp16/fp32)";
+    case DSA_KV_ERR_ALIGNMENT: return "misaligned pointer or stride (rows start on 16 bytes)";
+    case DSA_KV_ERR_UNSUPPORTED: return "sizes beyond the 32-bit index range of the kernel";
+    case DSA_KV_ERR_CUDA: return "a CUDA call failed";
+    case DSA_KV_ERR_BAD_ARGS_SIZE:
+      return "argument struct size mismatch (header and library differ) or reserved field not 0";
+    default: return "unknown dsa_kv status";
+  }
+}
+
+int dsa_kv_rope_launch(const dsa_kv_rope_args_t* a, void* stream) { return kv::rope(a, stream); }
+int dsa_kv_write_launch(const dsa_kv_copy_args_t* a, void* stream) { return kv::copy(a, stream, true); }
+int dsa_kv_read_launch(const dsa_kv_copy_args_t* a, void* stream) { return kv::copy(a, stream, false); }
+
+}  // extern "C"
