@@ -11,9 +11,11 @@ Also a drop-in for ``dsa_topk_page_table_transform``
 libdsa_topk.so (C ABI: include/dsa_topk.h).
 
 Around that selection, the quantised, paged KV cache (libdsa_kv.so, C ABI:
-include/dsa_kv.h): ``qk_rmsnorm_rope``, ``paged_kv_quant_write`` and
-``paged_kv_dequant_read``.
+include/dsa_kv.h): ``qk_rmsnorm_rope``, ``paged_kv_quant_write``,
+``paged_kv_dequant_read`` and, over the blocks that the selection names,
+``dsa_paged_attention``.
 """
+from .dsa_attention import dsa_paged_attention  # noqa: F401
 from .kv_cache import paged_kv_dequant_read, paged_kv_quant_write  # noqa: F401
 from .offload import fused_add_rmsnorm_group_quant_host  # noqa: F401
 from .qk_rope import qk_rmsnorm_rope  # noqa: F401
@@ -23,4 +25,4 @@ from . import task01, task02  # noqa: F401,E402
 
 __all__ = ["fused_add_rmsnorm_group_quant", "fused_add_rmsnorm_group_quant_host", "launch_plan",
            "dsa_topk_page_table_transform", "qk_rmsnorm_rope", "paged_kv_quant_write",
-           "paged_kv_dequant_read"]
+           "paged_kv_dequant_read", "dsa_paged_attention"]

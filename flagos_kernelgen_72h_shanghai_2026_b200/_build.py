@@ -27,7 +27,8 @@ TOPK_HEADERS = [INCLUDE_DIR / "dsa_topk.h", CSRC_DIR / "dsa_topk_kernel.cuh"]
 TOPK_LIB_PATH = PKG_DIR / "libdsa_topk.so"
 
 KV_SOURCES = sorted(CSRC_DIR.glob("dsa_kv*.cu"))
-KV_HEADERS = [INCLUDE_DIR / "dsa_kv.h", *sorted(CSRC_DIR.glob("kv_*.cuh"))]
+KV_HEADERS = [INCLUDE_DIR / "dsa_kv.h", *sorted(CSRC_DIR.glob("kv_*.cuh")),
+              CSRC_DIR / "kv_host.h", CSRC_DIR / "farq_kernel.cuh", INCLUDE_DIR / "farq.h"]
 KV_LIB_PATH = PKG_DIR / "libdsa_kv.so"
 
 OBJ_DIR = PKG_DIR / "_build"

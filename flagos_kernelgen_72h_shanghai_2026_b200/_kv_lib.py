@@ -87,10 +87,26 @@ class CopyArgs(ctypes.Structure):
     ]
 
 
+class AttnArgs(ctypes.Structure):
+    """Mirror of dsa_kv_attn_args_t."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("dtype", ctypes.c_int32),
+        ("block_dtype", ctypes.c_int32), ("page_dtype", ctypes.c_int32),
+        ("pos_dtype", ctypes.c_int32), ("softmax_scale", ctypes.c_float),
+        ("B", ctypes.c_int64), ("Q", ctypes.c_int64), ("G", ctypes.c_int64),
+        ("K", ctypes.c_int64),
+        ("q", Dense), ("out", Dense), ("cache", Cache),
+        ("blocks", ctypes.c_void_p), ("pages", ctypes.c_void_p),
+        ("blocks_stride", ctypes.c_int64 * 3), ("pages_stride", ctypes.c_int64 * 3),
+        ("q_pos", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 _LAUNCHES = {"dsa_kv_rope_launch": RopeArgs, "dsa_kv_write_launch": CopyArgs,
-             "dsa_kv_read_launch": CopyArgs}
+             "dsa_kv_read_launch": CopyArgs, "dsa_kv_attn_launch": AttnArgs}
 
 
 def load(path: Path | str | None = None) -> ctypes.CDLL:

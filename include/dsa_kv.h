@@ -9,6 +9,8 @@
  *                         scale per token and head, into their pages
  *   dsa_kv_read_launch    keys and values of whole sequences, back from their
  *                         pages as dense 16-bit tensors
+ *   dsa_kv_attn_launch    attention of every query row over the blocks that
+ *                         dsa_topk_page_table_transform selected for it
  * The reference project has none of them: its block selection ends with the
  * page ids, and the consumer of those ids is left to the caller.
  *
@@ -138,11 +140,46 @@ typedef struct dsa_kv_copy_args {
     const void* pos;              /* q_pos [B, Q] (write), kv_lens [B] (read)      */
 } dsa_kv_copy_args_t;
 
+/*
+ * Attention over selected blocks. q [B, Q, H * G, D]: query heads h * G to
+ * h * G + G - 1 share key head h and its selection. blocks, pages [B, H, Q, K]
+ * (as dsa_topk_launch writes them; the last dimension contiguous, strides in
+ * elements): entry i of a row stands for the tokens
+ *     t = blocks[i] * block_size + j,  0 <= j < block_size,
+ *     t <= q_pos[b, q],  t < kv_lens[b]
+ * whose keys and values lie in page pages[i]. An entry with a negative block
+ * id, or a page id outside [0, P), stands for none; one that occurs twice
+ * counts twice.
+ *     out = sum_t softmax(scale * q.k_t) v_t,   lse = ln sum_t exp(scale * q.k_t)
+ * A row without a token (and a padded one, q_pos < 0) has out = 0, lse = -inf.
+ * v_scale is positive; one below 1e-12, the least that a write leaves, counts
+ * as 1e-12.
+ * D is 64, 128 or 256, block_size >= 8.
+ */
+typedef struct dsa_kv_attn_args {
+    uint32_t struct_size;         /* = sizeof(dsa_kv_attn_args_t)                  */
+    int32_t  dtype;               /* BF16 | FP16: q, out                           */
+    int32_t  block_dtype;         /* INT32 | INT64: blocks                         */
+    int32_t  page_dtype;          /* INT32 | INT64: pages                          */
+    int32_t  pos_dtype;           /* INT32 | INT64: q_pos and kv_lens              */
+    float    softmax_scale;
+    int64_t  B, Q, G, K;
+    dsa_kv_dense_t q, out;
+    dsa_kv_cache_t cache;
+    const void* blocks;
+    const void* pages;
+    int64_t  blocks_stride[3], pages_stride[3];   /* b, h, q                       */
+    const void* q_pos;            /* [B, Q], contiguous                            */
+    const void* kv_lens;          /* [B]                                           */
+    float*   lse;                 /* [B, Q, H * G], contiguous; may be NULL        */
+} dsa_kv_attn_args_t;
+
 /* Each validates every argument before any device call and returns a
  * dsa_kv_status; on DSA_KV_OK the work is queued, not finished. */
 int dsa_kv_rope_launch(const dsa_kv_rope_args_t* args, void* stream);
 int dsa_kv_write_launch(const dsa_kv_copy_args_t* args, void* stream);
 int dsa_kv_read_launch(const dsa_kv_copy_args_t* args, void* stream);
+int dsa_kv_attn_launch(const dsa_kv_attn_args_t* args, void* stream);
 
 /* Static string for a dsa_kv_status (never NULL). */
 const char* dsa_kv_strerror(int status);

@@ -107,3 +107,41 @@ def paged_kv_dequant_read_ref(k_cache, k_scale, v_cache, v_scale, page_table, kv
                 out[b, t] = val[page, :, t % bs] if 0 <= page < P else 0.0
         got.append(out)
     return tuple(got)
+
+
+def dsa_paged_attention_ref(q, k_cache, k_scale, v_cache, v_scale, blocks, pages, q_pos, kv_lens, softmax_scale):
+    """dict of float64 tensors: out [B, Q, Hq, D], lse [B, Q, Hq], and what error bounds are made of, per row and
+    head: n, the number of tokens; score, the largest sum over D of the magnitudes of a score's terms; size [.., D],
+    the weighted sum of the values' magnitudes; top, the largest weight times value scale."""
+    P, H, bs, D = k_cache.shape
+    B, Q, Hq, _ = q.shape
+    G = Hq // H
+    shape = (B, Q, Hq)
+    r = {"out": torch.zeros(*shape, D, dtype=torch.float64), "lse": torch.full(shape, -math.inf, dtype=torch.float64),
+         "size": torch.zeros(*shape, D, dtype=torch.float64), "n": torch.zeros(shape, dtype=torch.float64),
+         "score": torch.zeros(shape, dtype=torch.float64), "top": torch.zeros(shape, dtype=torch.float64)}
+    kc, vc = k_cache.float().double(), v_cache.float().double()
+    for b in range(B):
+        for i in range(Q):
+            pos, n = int(q_pos[b, i]), int(kv_lens[b])
+            lim = min(pos + 1, n) if pos >= 0 else 0
+            for h in range(H):
+                where = []
+                for blk, page in zip(blocks[b, h, i].tolist(), pages[b, h, i].tolist()):
+                    if blk >= 0 and 0 <= page < P:
+                        where += [(page, j) for j in range(bs) if blk * bs + j < lim]
+                if not where:
+                    continue
+                pg, off = torch.tensor(where).T
+                ks, vs = k_scale[pg, h, off].double(), v_scale[pg, h, off].double()
+                k, v = kc[pg, h, off] * ks[:, None], vc[pg, h, off] * vs[:, None]
+                x = q[b, i, h * G:(h + 1) * G].double()
+                s = x @ k.T * softmax_scale
+                lse = torch.logsumexp(s, -1)
+                p = torch.exp(s - lse[:, None])
+                at = (b, i, slice(h * G, (h + 1) * G))
+                r["out"][at], r["lse"][at], r["size"][at] = p @ v, lse, p @ v.abs()
+                r["n"][at] = len(where)
+                r["score"][at] = (x.abs() @ k.abs().T * abs(softmax_scale)).amax(-1)
+                r["top"][at] = (p * vs).amax(-1)
+    return r

@@ -28,8 +28,8 @@ def lib():
 def test_library_exports_every_declared_symbol(lib):
     text = re.sub(r"/\*.*?\*/", "", HEADER.read_text(), flags=re.S)
     names = re.findall(r"^\s*(?:int|const char\*)\s+(dsa_kv_\w+)\s*\(", text, flags=re.M)
-    assert {"dsa_kv_rope_launch", "dsa_kv_write_launch", "dsa_kv_read_launch", "dsa_kv_strerror",
-            "dsa_kv_abi_version"} <= set(names)
+    assert {"dsa_kv_rope_launch", "dsa_kv_write_launch", "dsa_kv_read_launch", "dsa_kv_attn_launch",
+            "dsa_kv_strerror", "dsa_kv_abi_version"} <= set(names)
     raw = ctypes.CDLL(str(KV_LIB_PATH))
     for name in names:
         assert hasattr(raw, name), f"{name} declared in dsa_kv.h but not exported"
@@ -40,6 +40,7 @@ def test_struct_layout(lib):
     assert ctypes.sizeof(L.Cache) == 2 * 4 + 4 * 8 + 4 * 8 + 12 * 8
     assert ctypes.sizeof(L.RopeArgs) == 6 * 4 + 7 * 8 + 4 * 32 + 4 * 8
     assert ctypes.sizeof(L.CopyArgs) == 4 * 4 + 3 * 8 + 2 * 32 + ctypes.sizeof(L.Cache) + 2 * 8
+    assert ctypes.sizeof(L.AttnArgs) == 6 * 4 + 4 * 8 + 2 * 32 + ctypes.sizeof(L.Cache) + 2 * 8 + 6 * 8 + 3 * 8
     assert lib.dsa_kv_abi_version() == L.ABI_VERSION
     for code in range(0, 9):
         assert lib.dsa_kv_strerror(code)
@@ -78,6 +79,45 @@ def _copy(**kw):
     a.cache = L.Cache(L.DTYPE_E4M3, 0, 9, 2, 16, 128, 0x30000, 0x40000, 0x50000, 0x60000, s, s, ss, ss)
     a.page_table, a.pos = 0x70000, 0x80000
     return _set(a, kw)
+
+
+def _attn(**kw):
+    a = L.AttnArgs(struct_size=ctypes.sizeof(L.AttnArgs), dtype=L.DTYPE_FP16, block_dtype=L.DTYPE_INT32,
+                   page_dtype=L.DTYPE_INT64, pos_dtype=L.DTYPE_INT32, softmax_scale=0.1, B=2, Q=3, G=4, K=5)
+    three = ctypes.c_int64 * 3
+    a.q, a.out = L.Dense(0x10000, 3 * 1024, 1024, 128), L.Dense(0x20000, 3 * 1024, 1024, 128)
+    a.cache = _copy().cache
+    a.blocks, a.pages, a.q_pos, a.kv_lens, a.lse = 0x70000, 0x80000, 0x90000, 0xa0000, 0xb0000
+    a.blocks_stride = a.pages_stride = three(30, 15, 5)
+    return _set(a, kw)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(struct_size=8), L.ERR_BAD_ARGS_SIZE),
+    (dict(cache__reserved0=1), L.ERR_BAD_ARGS_SIZE),
+    (dict(dtype=L.DTYPE_E4M3), L.ERR_BAD_DTYPE),
+    (dict(block_dtype=L.DTYPE_FP32), L.ERR_BAD_DTYPE),
+    (dict(pos_dtype=9), L.ERR_BAD_DTYPE),
+    (dict(G=0), L.ERR_BAD_SHAPE),
+    (dict(K=-1), L.ERR_BAD_SHAPE),
+    (dict(cache__D=96), L.ERR_BAD_HEAD_DIM),
+    (dict(cache__block_size=7), L.ERR_BAD_HEAD_DIM),
+    (dict(cache__block_size=65537), L.ERR_UNSUPPORTED),
+    (dict(B=1 << 20, Q=1 << 10), L.ERR_UNSUPPORTED),
+    (dict(K=1 << 31), L.ERR_UNSUPPORTED),
+    (dict(K=1 << 29, cache__block_size=4096), L.ERR_UNSUPPORTED),
+    (dict(blocks=0), L.ERR_NULL_POINTER),
+    (dict(kv_lens=0), L.ERR_NULL_POINTER),
+    (dict(q__ptr=0), L.ERR_NULL_POINTER),
+    (dict(cache__k_scale=0), L.ERR_NULL_POINTER),
+    (dict(q__ptr=0x10002), L.ERR_ALIGNMENT),
+    (dict(out__stride_h=0), L.ERR_BAD_SHAPE),
+    (dict(pages=0x80004), L.ERR_ALIGNMENT),
+    (dict(lse=0xb0002), L.ERR_ALIGNMENT),
+    (dict(cache__v_codes=0x40004), L.ERR_ALIGNMENT),
+])
+def test_attention_validation_before_any_device_call(lib, kw, code):
+    assert lib.dsa_kv_attn_launch(ctypes.byref(_attn(**kw)), None) == code
 
 
 @pytest.mark.parametrize("kw,code", [
@@ -154,6 +194,8 @@ def test_empty_calls_are_no_ops(lib):
         assert entry(ctypes.byref(_copy(Q=0, k__ptr=0)), None) == L.OK
         assert entry(ctypes.byref(_copy(NB=0, page_table=0)), None) == L.OK
     assert lib.dsa_kv_write_launch(ctypes.byref(_copy(cache__P=0)), None) == L.OK
+    assert lib.dsa_kv_attn_launch(ctypes.byref(_attn(B=0)), None) == L.OK
+    assert lib.dsa_kv_attn_launch(ctypes.byref(_attn(Q=0, q__ptr=0)), None) == L.OK
 
 
 def test_wrappers_refuse_cpu_tensors():
@@ -167,6 +209,9 @@ def test_wrappers_refuse_cpu_tensors():
         pkg.paged_kv_quant_write(k, k, *c, table, pos)
     with pytest.raises(TypeError, match="CUDA"):
         pkg.paged_kv_dequant_read(*c, table, pos[0, :1], k, k)
+    sel = torch.zeros(1, 2, 2, 1, dtype=torch.int32)
+    with pytest.raises(TypeError, match="CUDA"):
+        pkg.dsa_paged_attention(q.half(), *c, sel, sel, pos, pos[0, :1], q.half(), None, 0.1)
     with pytest.raises(TypeError, match="torch.Tensor"):
         pkg.paged_kv_quant_write(None, k, *c, table, pos)
 
@@ -214,6 +259,33 @@ def test_oracle_read_after_write_is_within_half_a_step():
         ko, vo = R.paged_kv_dequant_read_ref(kc.view(dt), ks, vc.view(dt), vs, table, torch.tensor([40]), k, v)
         for got, x in ((ko, k), (vo, v)):
             assert ((got - x).abs() <= step * x.abs().amax(-1, keepdim=True) * (1 + 1e-6)).all()
+
+
+def test_oracle_attention_against_a_dense_softmax():
+    """All blocks selected, one of them twice by mistake of nobody: the oracle against torch's softmax on the dense
+    context, with the doubled block's tokens in it twice."""
+    g = gen(4)
+    B, Q, H, G, D, bs, NB = 2, 3, 2, 2, 16, 8, 4
+    table, P = page_table(g, B, NB)
+    c = caches(g, P, H, bs, D, torch.int8)
+    q = torch.randn(B, Q, H * G, D, generator=g)
+    lens = torch.tensor([29, 17])
+    pos = lens[:, None] - Q + torch.arange(Q)
+    order = torch.tensor([2, 0, 3, 1, 0])
+    blocks = order.expand(B, H, Q, 5)
+    pages = table.long()[:, order][:, None, None].expand(B, H, Q, 5)
+    r = R.dsa_paged_attention_ref(q, *c, blocks, pages, pos, lens, 0.3)
+    zero = torch.zeros(B, NB * bs, H, D)
+    k, v = R.paged_kv_dequant_read_ref(*c, table, torch.full((B,), NB * bs), zero, zero)
+    at = torch.arange(NB * bs)
+    for b in range(B):
+        for i in range(Q):
+            for x in range(H * G):
+                s = k[b, :, x // G] @ q[b, i, x].double() * 0.3 + torch.log((at < bs).double() + 1)
+                s = s.masked_fill((at > pos[b, i]) | (at >= lens[b]), float("-inf"))
+                want = torch.softmax(s, 0) @ v[b, :, x // G]
+                assert torch.allclose(r["out"][b, i, x], want, atol=1e-12)
+                assert abs(float(r["lse"][b, i, x] - torch.logsumexp(s, 0))) < 1e-12
 
 
 def test_index_division_by_multiplication():
