@@ -104,10 +104,11 @@ def fast_ext_path() -> Path:
 
 def build_fast_ext(force: bool = False, verbose: bool = False) -> Path:
     """Compile the C++ launch path of the Python operators (_farq_fast, a
-    torch extension module linked against libfarq.so and libdsa_topk.so)
-    with g++, in-tree, if it is missing or older than its sources."""
+    torch extension module linked against libfarq.so, libdsa_topk.so and
+    libdsa_kv.so) with g++, in-tree, if it is missing or older than its sources."""
     out = fast_ext_path()
-    deps = [FAST_SOURCE, INCLUDE_DIR / "farq.h", INCLUDE_DIR / "dsa_topk.h", LIB_PATH, TOPK_LIB_PATH]
+    deps = [FAST_SOURCE, INCLUDE_DIR / "farq.h", INCLUDE_DIR / "dsa_topk.h",
+            INCLUDE_DIR / "dsa_kv.h", LIB_PATH, TOPK_LIB_PATH, KV_LIB_PATH]
     if not force and not _stale(out, deps):
         return out
     import sysconfig
@@ -125,7 +126,7 @@ def build_fast_ext(force: bool = False, verbose: bool = False) -> Path:
            str(FAST_SOURCE), "-o", str(out) + ".tmp",
            *[f"-L{p}" for p in cpp_extension.library_paths()],
            "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
-           f"-L{PKG_DIR}", "-lfarq", "-ldsa_topk",
+           f"-L{PKG_DIR}", "-lfarq", "-ldsa_topk", "-ldsa_kv",
            "-Wl,-rpath,$ORIGIN", *[f"-Wl,-rpath,{p}" for p in cpp_extension.library_paths()]]
     _run(cmd, verbose)
     os.replace(str(out) + ".tmp", out)

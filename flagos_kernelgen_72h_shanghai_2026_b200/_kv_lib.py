@@ -16,6 +16,11 @@ import torch
 
 from ._build import KV_LIB_PATH
 
+try:  # C++ launch path (csrc/farq_fast.cpp); without it every call takes the ctypes path
+    from . import _farq_fast as _fast
+except ImportError:
+    _fast = None
+
 # enum dsa_kv_dtype
 DTYPE_BF16, DTYPE_FP16, DTYPE_FP32, DTYPE_INT8, DTYPE_E4M3, DTYPE_INT32, DTYPE_INT64 = range(7)
 
@@ -151,6 +156,22 @@ def raise_status(op: str, status: int):
     if status in (ERR_CUDA, ERR_BAD_ARGS_SIZE):
         raise RuntimeError(msg)
     raise ValueError(msg)
+
+
+def fast_launch(op: str, entry: str, tensors: tuple, *args) -> bool:
+    """Hand the call to the C++ launch path; False when it declines (it has then launched nothing)."""
+    if _fast is None:
+        return False
+    for t in tensors:
+        if type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
+            return False
+    try:
+        st = getattr(_fast, entry)(*tensors, *args)
+    except TypeError:  # a scalar pybind11 cannot convert: the checks of the Python path report it
+        return False
+    if st > 0:
+        raise_status(op, st)
+    return st == OK
 
 
 def launch(op: str, entry: str, args, device: torch.device) -> None:

@@ -1,18 +1,21 @@
-// farq_fast.cpp — C++ launch path of the two Python operators.
+// farq_fast.cpp — C++ launch path of the Python operators.
 //
-// The Python wrappers (task01.py, task02.py) check tensors and fill the C
-// argument structs in Python, which costs about 10 us per call — more than
-// the kernel itself for a few rows (the reference's small-M regime,
+// The Python wrappers (task01.py, task02.py, qk_rope.py, kv_cache.py,
+// dsa_attention.py) check tensors and fill the C argument structs in Python,
+// which costs 10 to 25 us per call — more than the kernel itself for a few
+// rows (the reference's small-M regime,
 // reports/task01_fused_add_rmsnorm_group_quant.md:57). This extension does the
 // same checks and the struct fill in C++ for the common case (contiguous
-// tensors on one CUDA device) and calls the same plain-C entry points
-// (farq_launch, dsa_topk_launch) on the current stream. Anything else — an
+// tensors on one CUDA device; strided ones too for the operators of the paged
+// cache) and calls the same plain-C entry points (farq_launch,
+// dsa_topk_launch, dsa_kv_*_launch) on the current stream. Anything else — an
 // unusual layout, a bad argument — returns -1 without launching, and the
 // Python path handles the call (and raises its precise error).
 #include <torch/extension.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include "dsa_kv.h"
 #include "dsa_topk.h"
 #include "farq.h"
 
@@ -145,10 +148,182 @@ int64_t task02(const at::Tensor& scores, const at::Tensor& page_table, const at:
   return dsa_topk_launch(&a, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
 }
 
+// ------------------------------------------------------------ the paged cache
+int half_code(at::ScalarType t) {
+  return t == at::kBFloat16 ? DSA_KV_BF16 : t == at::kHalf ? DSA_KV_FP16 : -1;
+}
+int kv_index_code(at::ScalarType t) {
+  return t == at::kInt ? DSA_KV_INT32 : t == at::kLong ? DSA_KV_INT64 : -1;
+}
+bool on(const at::Tensor& t, const at::Device& dev) { return t.defined() && t.device() == dev; }
+
+// A [B, Q, H, D] tensor whose last dimension is contiguous.
+bool dense4(const at::Tensor& t, int64_t B, int64_t Q, int64_t H, int64_t D, at::ScalarType type,
+            const at::Device& dev, dsa_kv_dense_t* d) {
+  if (!on(t, dev) || t.scalar_type() != type || t.dim() != 4 || t.size(0) != B || t.size(1) != Q ||
+      t.size(2) != H || t.size(3) != D || (D > 1 && t.stride(3) != 1))
+    return false;
+  d->ptr = t.data_ptr();
+  d->stride_b = t.stride(0);
+  d->stride_q = t.stride(1);
+  d->stride_h = t.stride(2);
+  return true;
+}
+
+bool cache_of(const at::Tensor& kc, const at::Tensor& ks, const at::Tensor& vc, const at::Tensor& vs,
+              const at::Device& dev, dsa_kv_cache_t* c) {
+  if (!on(kc, dev) || !on(ks, dev) || !on(vc, dev) || !on(vs, dev)) return false;
+  const at::ScalarType t = kc.scalar_type();
+  if ((t != at::kChar && t != at::kFloat8_e4m3fn) || vc.scalar_type() != t || ks.scalar_type() != at::kFloat ||
+      vs.scalar_type() != at::kFloat || kc.dim() != 4 || ks.dim() != 3 || vs.dim() != 3 || vc.sizes() != kc.sizes() ||
+      ks.sizes() != kc.sizes().slice(0, 3) || vs.sizes() != ks.sizes())
+    return false;
+  if (kc.size(3) > 1 && (kc.stride(3) != 1 || vc.stride(3) != 1)) return false;
+  c->code_dtype = t == at::kChar ? DSA_KV_INT8 : DSA_KV_E4M3;
+  c->reserved0 = 0;
+  c->P = kc.size(0);
+  c->H = kc.size(1);
+  c->block_size = kc.size(2);
+  c->D = kc.size(3);
+  c->k_codes = kc.data_ptr();
+  c->v_codes = vc.data_ptr();
+  c->k_scale = ks.data_ptr<float>();
+  c->v_scale = vs.data_ptr<float>();
+  for (int i = 0; i < 3; ++i) {
+    c->k_stride[i] = kc.stride(i);
+    c->v_stride[i] = vc.stride(i);
+    c->k_scale_stride[i] = ks.stride(i);
+    c->v_scale_stride[i] = vs.stride(i);
+  }
+  return true;
+}
+
+// qk_rmsnorm_rope (qk_rope.py); returns dsa_kv_rope_launch's status or kNotHandled.
+int64_t kv_rope(const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_gamma, const at::Tensor& k_gamma,
+                const at::Tensor& cos_sin, const at::Tensor& positions, const at::Tensor& q_out,
+                const at::Tensor& k_out, double eps, bool interleaved) {
+  if (!q.defined() || !q.is_cuda() || q.dim() != 4 || !k.defined() || k.dim() != 4) return kNotHandled;
+  const at::Device dev = q.device();
+  dsa_kv_rope_args_t a = {};
+  a.struct_size = sizeof(a);
+  a.B = q.size(0);
+  a.Q = q.size(1);
+  a.Hq = q.size(2);
+  a.Hk = k.size(2);
+  a.D = q.size(3);
+  const at::ScalarType t = q.scalar_type();
+  a.dtype = half_code(t);
+  if (a.dtype < 0 || !dense4(q, a.B, a.Q, a.Hq, a.D, t, dev, &a.q) || !dense4(k, a.B, a.Q, a.Hk, a.D, t, dev, &a.k) ||
+      !dense4(q_out, a.B, a.Q, a.Hq, a.D, t, dev, &a.q_out) || !dense4(k_out, a.B, a.Q, a.Hk, a.D, t, dev, &a.k_out))
+    return kNotHandled;
+  if (!same_cuda(q_gamma, dev) || !same_cuda(k_gamma, dev) || !same_cuda(cos_sin, dev) || !same_cuda(positions, dev))
+    return kNotHandled;
+  const at::ScalarType gt = q_gamma.scalar_type();
+  a.gamma_dtype = gt == at::kFloat ? DSA_KV_FP32 : half_code(gt);
+  a.pos_dtype = kv_index_code(positions.scalar_type());
+  if (a.gamma_dtype < 0 || a.pos_dtype < 0 || k_gamma.scalar_type() != gt || q_gamma.dim() != 1 ||
+      q_gamma.size(0) != a.D || k_gamma.dim() != 1 || k_gamma.size(0) != a.D || cos_sin.dim() != 2 ||
+      cos_sin.scalar_type() != at::kFloat || !is_2d(positions, a.B, a.Q))
+    return kNotHandled;
+  a.max_pos = cos_sin.size(0);
+  a.rot = cos_sin.size(1);
+  a.interleaved = interleaved ? 1 : 0;
+  a.eps = (float)eps;
+  a.q_gamma = q_gamma.data_ptr();
+  a.k_gamma = k_gamma.data_ptr();
+  a.cos_sin = cos_sin.data_ptr<float>();
+  a.positions = positions.data_ptr();
+  const c10::cuda::CUDAGuard guard(dev);
+  return dsa_kv_rope_launch(&a, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+}
+
+// paged_kv_quant_write and paged_kv_dequant_read (kv_cache.py); returns the
+// entry point's status or kNotHandled.
+int64_t kv_copy(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& k_scale,
+                const at::Tensor& v_cache, const at::Tensor& v_scale, const at::Tensor& page_table,
+                const at::Tensor& pos, bool write) {
+  if (!k.defined() || !k.is_cuda() || k.dim() != 4) return kNotHandled;
+  const at::Device dev = k.device();
+  dsa_kv_copy_args_t a = {};
+  a.struct_size = sizeof(a);
+  if (!cache_of(k_cache, k_scale, v_cache, v_scale, dev, &a.cache)) return kNotHandled;
+  a.B = k.size(0);
+  a.Q = k.size(1);
+  const at::ScalarType t = k.scalar_type();
+  a.dtype = half_code(t);
+  if (a.dtype < 0 || !dense4(k, a.B, a.Q, a.cache.H, a.cache.D, t, dev, &a.k) ||
+      !dense4(v, a.B, a.Q, a.cache.H, a.cache.D, t, dev, &a.v) || !same_cuda(page_table, dev) || !same_cuda(pos, dev))
+    return kNotHandled;
+  a.page_dtype = kv_index_code(page_table.scalar_type());
+  a.pos_dtype = kv_index_code(pos.scalar_type());
+  if (a.page_dtype < 0 || a.pos_dtype < 0 || page_table.dim() != 2 || page_table.size(0) != a.B) return kNotHandled;
+  if (write ? !is_2d(pos, a.B, a.Q) : pos.dim() != 1 || pos.size(0) != a.B) return kNotHandled;
+  a.NB = page_table.size(1);
+  a.page_table = page_table.data_ptr();
+  a.pos = pos.data_ptr();
+  const c10::cuda::CUDAGuard guard(dev);
+  void* stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  return write ? dsa_kv_write_launch(&a, stream) : dsa_kv_read_launch(&a, stream);
+}
+
+bool selection(const at::Tensor& t, const dsa_kv_attn_args_t& a, const at::Device& dev, int32_t* code, int64_t s[3]) {
+  if (!on(t, dev) || t.dim() != 4 || t.size(0) != a.B || t.size(1) != a.cache.H || t.size(2) != a.Q ||
+      t.size(3) != a.K || (a.K > 1 && t.stride(3) != 1))
+    return false;
+  *code = kv_index_code(t.scalar_type());
+  for (int i = 0; i < 3; ++i) s[i] = t.stride(i);
+  return *code >= 0;
+}
+
+// dsa_paged_attention (dsa_attention.py); returns dsa_kv_attn_launch's status or kNotHandled.
+int64_t kv_attn(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& k_scale, const at::Tensor& v_cache,
+                const at::Tensor& v_scale, const at::Tensor& blocks, const at::Tensor& pages, const at::Tensor& q_pos,
+                const at::Tensor& kv_lens, const at::Tensor& out, const c10::optional<at::Tensor>& lse,
+                double softmax_scale) {
+  if (!q.defined() || !q.is_cuda() || q.dim() != 4 || !blocks.defined() || blocks.dim() != 4) return kNotHandled;
+  const at::Device dev = q.device();
+  dsa_kv_attn_args_t a = {};
+  a.struct_size = sizeof(a);
+  if (!cache_of(k_cache, k_scale, v_cache, v_scale, dev, &a.cache)) return kNotHandled;
+  const int64_t Hq = q.size(2), H = a.cache.H;
+  if (H < 1 || Hq < 1 || Hq % H != 0) return kNotHandled;
+  a.B = q.size(0);
+  a.Q = q.size(1);
+  a.G = Hq / H;
+  a.K = blocks.size(3);
+  const at::ScalarType t = q.scalar_type();
+  a.dtype = half_code(t);
+  if (a.dtype < 0 || !dense4(q, a.B, a.Q, Hq, a.cache.D, t, dev, &a.q) ||
+      !dense4(out, a.B, a.Q, Hq, a.cache.D, t, dev, &a.out) ||
+      !selection(blocks, a, dev, &a.block_dtype, a.blocks_stride) ||
+      !selection(pages, a, dev, &a.page_dtype, a.pages_stride) || !same_cuda(q_pos, dev) || !same_cuda(kv_lens, dev))
+    return kNotHandled;
+  a.pos_dtype = kv_index_code(q_pos.scalar_type());
+  if (a.pos_dtype < 0 || kv_lens.scalar_type() != q_pos.scalar_type() || !is_2d(q_pos, a.B, a.Q) ||
+      kv_lens.dim() != 1 || kv_lens.size(0) != a.B)
+    return kNotHandled;
+  if (lse.has_value()) {
+    if (!same_cuda(*lse, dev) || lse->scalar_type() != at::kFloat || lse->dim() != 3 || lse->size(0) != a.B ||
+        lse->size(1) != a.Q || lse->size(2) != Hq)
+      return kNotHandled;
+    a.lse = lse->data_ptr<float>();
+  }
+  a.softmax_scale = (float)softmax_scale;
+  a.blocks = blocks.data_ptr();
+  a.pages = pages.data_ptr();
+  a.q_pos = q_pos.data_ptr();
+  a.kv_lens = kv_lens.data_ptr();
+  const c10::cuda::CUDAGuard guard(dev);
+  return dsa_kv_attn_launch(&a, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-  m.doc() = "C++ launch path of fused_add_rmsnorm_group_quant and dsa_topk_page_table_transform";
+  m.doc() = "C++ launch path of the Python operators";
   m.def("task01", &task01, "checks + farq_launch; status, or -1 when not handled");
   m.def("task02", &task02, "checks + dsa_topk_launch; status, or -1 when not handled");
+  m.def("kv_rope", &kv_rope, "checks + dsa_kv_rope_launch; status, or -1 when not handled");
+  m.def("kv_copy", &kv_copy, "checks + dsa_kv_write_launch / dsa_kv_read_launch; status, or -1 when not handled");
+  m.def("kv_attn", &kv_attn, "checks + dsa_kv_attn_launch; status, or -1 when not handled");
 }

@@ -18,6 +18,8 @@ import torch
 
 from . import _kv_lib as L
 
+_OP = "dsa_paged_attention"
+
 
 def _selection(name, t, device, shape):
     L.check_tensor(name, t, device)
@@ -47,6 +49,9 @@ def dsa_paged_attention(q: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.T
     padded one (negative position), has out = 0 and lse = -inf.
 
     D is 64, 128 or 256; block_size is 8 to 65536."""
+    if L.fast_launch(_OP, "kv_attn", (q, k_cache, k_scale, v_cache, v_scale, blocks, pages, q_pos,
+                                      kv_lens, out), lse, softmax_scale):
+        return out, lse
     dev = L.check_tensor("q", q, None)
     a = L.AttnArgs()
     a.struct_size = ctypes.sizeof(a)
@@ -91,5 +96,5 @@ def dsa_paged_attention(q: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.T
     a.pages = pages.data_ptr() or None
     a.q_pos = q_pos.data_ptr() or None
     a.kv_lens = kv_lens.data_ptr() or None
-    L.launch("dsa_paged_attention", "dsa_kv_attn_launch", a, dev)
+    L.launch(_OP, "dsa_kv_attn_launch", a, dev)
     return out, lse

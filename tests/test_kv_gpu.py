@@ -10,8 +10,8 @@ import pytest
 import torch
 
 from oracle import kv_oracle as R
-from flagos_kernelgen_72h_shanghai_2026_b200 import (paged_kv_dequant_read, paged_kv_quant_write,
-                                                     qk_rmsnorm_rope)
+from flagos_kernelgen_72h_shanghai_2026_b200 import (_kv_lib, dsa_paged_attention, paged_kv_dequant_read,
+                                                     paged_kv_quant_write, qk_rmsnorm_rope)
 from _kv_cases import angles, caches, gen, layout, page_table
 
 pytestmark = pytest.mark.gpu
@@ -297,3 +297,71 @@ def test_write_and_read_on_a_side_stream_and_in_a_graph(dev):
         torch.cuda.synchronize(dev)
         for got, exact in zip((ko, vo), want):
             check_rounded(got, exact, U * exact.abs(), f"replay {n}")
+
+
+# ------------------------------------------------------------ C++ launch path
+def test_both_launch_paths_give_the_same_bytes(dev):
+    """The C++ launch path takes every one of these calls (strided inputs and parameters among them) and gives what
+    the ctypes path gives."""
+    from flagos_kernelgen_72h_shanghai_2026_b200._build import build_fast_ext
+    build_fast_ext()
+    fast = _kv_lib._fast
+    assert fast is not None, "C++ launch path not loaded"
+    g = gen(19)
+    B, Q, Hq, H, D, bs, NB = 2, 3, 4, 2, 64, 16, 3
+    table, P = page_table(g, B, NB)
+    c = caches(g, P, H, bs, D, E4M3)
+    q, k, gq, gk, _ = rope_inputs(B, Q, Hq, H, D, BF16, FP32, seed=20)
+    lens = torch.tensor([40, 30], dtype=torch.int32)
+    pos = (lens[:, None] - Q + torch.arange(Q)).int()
+    cs, td, pd, ld, qd, kd = (t.to(dev) for t in (angles(48, D), table, pos, lens, q, k))
+    params = tuple(torch.nn.Parameter(t.to(dev), requires_grad=False) for t in (gq, gk))
+    blocks = torch.arange(NB, dtype=torch.int32, device=dev).expand(B, H, Q, NB)
+    pages = td[:, None, None, :].expand(B, H, Q, NB)
+
+    def layer():
+        cd = to_dev(c, dev, "nhd")
+        qo, ko = torch.empty(B, Q, Hq, D, dtype=BF16, device=dev), torch.empty(B, Q, H, D, dtype=BF16, device=dev)
+        out, lse = torch.empty_like(qo), torch.empty(B, Q, Hq, device=dev)
+        k2, v2 = (torch.zeros(B, 48, H, D, dtype=BF16, device=dev) for _ in range(2))
+        qk_rmsnorm_rope(qd, kd, *params, cs, pd, qo, ko, 1e-6)
+        paged_kv_quant_write(ko, kd, *cd, td, pd)
+        dsa_paged_attention(qo, *cd, blocks, pages, pd, ld, out, lse, 0.1)
+        paged_kv_dequant_read(*cd, td, ld, k2, v2)
+        torch.cuda.synchronize(dev)
+        return [t.cpu() for t in (qo, ko, *cd, out, lse, k2, v2)]
+
+    class Counting:
+        def __init__(self):
+            self.ok = []
+
+        def __getattr__(self, name):
+            def call(*a):
+                self.ok.append(getattr(fast, name)(*a))
+                return self.ok[-1]
+            return call
+
+    counting = Counting()
+    try:
+        _kv_lib._fast = counting
+        a = layer()
+        _kv_lib._fast = None
+        b = layer()
+    finally:
+        _kv_lib._fast = fast
+    assert counting.ok == [0, 0, 0, 0]
+    assert all(same_bytes(x, y) for x, y in zip(a, b))
+
+
+def test_the_c_launch_path_declines_what_it_does_not_take(dev):
+    from flagos_kernelgen_72h_shanghai_2026_b200._build import build_fast_ext
+    build_fast_ext()
+    k = torch.zeros(1, 2, 2, 64, dtype=BF16, device=dev)
+    c = to_dev(caches(gen(1), 3, 2, 16, 64, E4M3), dev)
+    table, pos = torch.zeros(1, 2, dtype=torch.int32, device=dev), torch.zeros(1, 2, dtype=torch.int32, device=dev)
+    fast = _kv_lib._fast
+    assert fast.kv_copy(k, k, *c, table, pos, True) == 0
+    for bad in ((k.float(), k, *c, table, pos), (k.cpu(), k, *c, table, pos), (k, k[:, :1], *c, table, pos),
+                (k, k, *c, table.float(), pos), (k, k, *c, table, pos[0]), (k, k, c[0], c[1], c[2].view(INT8), c[3], table, pos)):
+        assert fast.kv_copy(*bad, True) == -1
+    torch.cuda.synchronize(dev)
