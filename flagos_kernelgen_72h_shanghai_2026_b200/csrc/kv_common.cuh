@@ -78,6 +78,30 @@ __device__ __forceinline__ uint2 ld_stream8(const void* p) {
   return v;
 }
 
+// ------------------------------------------------------------- fp32 pairs
+// Two fp32 values in one register pair: one instruction for both.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 both(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // ------------------------------------------------------------ 16-bit formats
 template <typename T>
 struct Half16;
@@ -137,18 +161,19 @@ __device__ __forceinline__ uint32_t to_s8(float v) { return (uint32_t)__float2in
 __device__ __forceinline__ uint32_t to_s8x4(float a, float b, float c, float d) {
   return to_s8(a) | (to_s8(b) << 8) | (to_s8(c) << 16) | (to_s8(d) << 24);
 }
-// Four codes as four fp32 values.
+// Four codes as two pairs of fp32 values.
 template <bool E4M3>
-__device__ __forceinline__ void decode4(uint32_t w, float f[4]) {
+__device__ __forceinline__ void decode4(uint32_t w, f32x2& lo, f32x2& hi) {
   if (E4M3) {
-    const uint32_t lo = e4m3x2_to_half2((uint16_t)w), hi = e4m3x2_to_half2((uint16_t)(w >> 16));
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+    const uint32_t a = e4m3x2_to_half2((uint16_t)w), b = e4m3x2_to_half2((uint16_t)(w >> 16));
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a));
+    const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&b));
+    lo = pair(x.x, x.y);
+    hi = pair(y.x, y.y);
   } else {
     const int v = (int)w;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = (float)(int8_t)(v >> (8 * i));
+    lo = pair((float)(int8_t)v, (float)(int8_t)(v >> 8));
+    hi = pair((float)(int8_t)(v >> 16), (float)(v >> 24));
   }
 }
 

@@ -370,7 +370,7 @@ def check_layer(dev, B, Q, Hq, H, D, bs, NB, K, code, graph):
     qc, kc, vc = (t.view(B, Q, -1, D) for t in qkv.split([Hq * D, H * D, H * D], dim=-1))
     (we, wsize), (ke, ksize) = R.qk_rmsnorm_rope_ref(qc, kc, gq, gk, cs, pos, qc, kc, 1e-6)
     for got, exact, size in ((qo, we, wsize), (ko, ke, ksize)):
-        tol = 2.0 ** -8 * (exact.abs() + 13 * U * size) + 13 * U * size
+        tol = 2.0 ** -8 * (exact.abs() + 14 * U * size) + 14 * U * size
         assert ((got.cpu().double() - exact).abs() <= tol).all()
     written = R.paged_kv_quant_write_ref(ko.cpu(), vc, *c, table, pos)
     for got, want in zip(cd, written):

@@ -66,10 +66,11 @@ def check_rope(dev, q, k, gq, gk, cs, pos, eps=1e-6, interleaved=False, in_place
     torch.cuda.synchronize(dev)
     want = R.qk_rmsnorm_rope_ref(q, k, gq, gk, cs, pos, old_q, old_k, eps, interleaved)
     for got, (exact, size), what in zip(out, want, "qk"):
-        # sum of squares: 8 products by fma in a lane, 5 sums across lanes, all terms positive: 13 u; times 1/D
-        # (rounded: u) plus eps by fma (u): 15 u; its root halves that: 7.5 u, its own rounding u; times x and
-        # times gamma u each: 10.5 u of every normed value; two products and their sum: 2 u more. 13 u of the terms.
-        check_rounded(got, exact, 13 * U * size, what)
+        # sum of squares: 4 products by fma into each of two sums, 6 sums across them and the lanes, all terms
+        # positive: 10 u; times 1/D (rounded: u) plus eps by fma (u): 12 u; its root halves that: 6 u, rsqrt's 2 ulp
+        # are at most 4 u: 10 u. gamma times cosine or sine u, times x u, the sum of the two products by fma u, times
+        # the root u: 14 u of the terms.
+        check_rounded(got, exact, 14 * U * size, what)
 
 
 @pytest.mark.parametrize("B,Q,Hq,Hk,D,rot,dtype,gdt,inter", [
