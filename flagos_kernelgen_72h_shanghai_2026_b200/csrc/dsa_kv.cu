@@ -108,7 +108,7 @@ int rope(const dsa_kv_rope_args_t* a, void* stream) {
   const RopeFn fn = a->dtype == DSA_KV_BF16
                         ? (a->interleaved ? rope_fn<__nv_bfloat16, true>(lanes) : rope_fn<__nv_bfloat16, false>(lanes))
                         : (a->interleaved ? rope_fn<__half, true>(lanes) : rope_fn<__half, false>(lanes));
-  return launch(fn, ceil_div(p.tasks, kCtaWarps), kCtaThreads, 0, stream, p);
+  return launch(fn, ceil_div(p.tasks, kCtaWarps), kCtaThreads, 0, 1, stream, p);
 }
 
 int copy(const dsa_kv_copy_args_t* a, void* stream, bool write) {
@@ -165,7 +165,7 @@ int copy(const dsa_kv_copy_args_t* a, void* stream, bool write) {
   const CopyFn fn = a->dtype == DSA_KV_BF16
                         ? (e ? copy_fn<__nv_bfloat16, true>(lanes, write, u) : copy_fn<__nv_bfloat16, false>(lanes, write, u))
                         : (e ? copy_fn<__half, true>(lanes, write, u) : copy_fn<__half, false>(lanes, write, u));
-  return launch(fn, ceil_div(p.tasks, kCtaWarps), kCtaThreads, 0, stream, p);
+  return launch(fn, ceil_div(p.tasks, kCtaWarps), kCtaThreads, 0, 1, stream, p);
 }
 
 }  // namespace kv

@@ -46,25 +46,32 @@ bool make_map(CUtensorMap* map, const dsa_kv_cache_t& c, void* codes, const int6
 }
 
 using AttnFn = void (*)(const AttnParams, const CUtensorMap, const CUtensorMap);
+
 struct Variant {
   AttnFn fn;
-  size_t smem;
+  size_t smem, more;  // shared memory of a CTA alone, and for each further CTA of its cluster
+  int tok, ctas;      // tokens of a chunk, CTAs per SM
 };
-
-// Ring slots per warp: as many as two CTAs per SM (D <= 128) or one have room for.
-constexpr int slots_of(int D) { return D == 64 ? 6 : 3; }
-
+template <typename T, bool E, int D, int NB, int TOK, int CTAS>
+Variant variant() {
+  using L = AttnSmem<D, NB, TOK>;
+  return Variant{attn_kernel<T, D, E, NB, TOK, CTAS>, L::total(1), L::total(2) - L::total(1), TOK, CTAS};
+}
+// Tokens of a chunk and CTAs per SM. A ring of three boxes of 64 tokens leaves
+// room for two CTAs at D = 128. Measured there with 16 heads (us, 1024 rows x
+// 2048 tokens): 64 tokens and 2 CTAs 95.7, 32 tokens and 3 CTAs 108.5, 32
+// tokens and 2 CTAs 118: what a chunk costs besides its products weighs more
+// than the warps that hide it.
 template <typename T, bool E>
-Variant variant_of(int64_t D) {
-  switch (D) {
-    case 64: return {attn_kernel<T, 64, E, slots_of(64)>, AttnSmem<64, slots_of(64)>::total};
-    case 128: return {attn_kernel<T, 128, E, slots_of(128)>, AttnSmem<128, slots_of(128)>::total};
-    default: return {attn_kernel<T, 256, E, slots_of(256)>, AttnSmem<256, slots_of(256)>::total};
-  }
+Variant variant_of(int64_t D, int nb) {
+  if (D == 64) return nb == 1 ? variant<T, E, 64, 1, 64, 3>() : variant<T, E, 64, 2, 64, 2>();
+  if (D == 128) return nb == 1 ? variant<T, E, 128, 1, 64, 2>() : variant<T, E, 128, 2, 64, 2>();
+  return nb == 1 ? variant<T, E, 256, 1, 32, 2>() : variant<T, E, 256, 2, 32, 1>();
 }
 
+std::atomic<int> g_sm_count[kMaxDevices];
 // Shared memory granted to each variant, per device.
-std::atomic<bool> g_granted[kMaxDevices][12];
+std::atomic<bool> g_granted[kMaxDevices][24];
 
 int attn(const dsa_kv_attn_args_t* a, void* stream) {
   if (!a) return DSA_KV_ERR_NULL_POINTER;
@@ -77,7 +84,11 @@ int attn(const dsa_kv_attn_args_t* a, void* stream) {
   const dsa_kv_cache_t& c = a->cache;
   if ((c.D != 64 && c.D != 128 && c.D != 256) || c.block_size < 8) return DSA_KV_ERR_BAD_HEAD_DIM;
   if (c.block_size > kMaxBlockSize || a->G > kMaxIndex) return DSA_KV_ERR_UNSUPPORTED;
-  const int64_t MT = ceil_div(a->G, kRows);
+  const int64_t n[3] = {c.P, c.H, c.block_size};
+  for (int i = 0; i < 3; ++i)  // the kernel holds the scales' strides in 32 bits
+    if (n[i] > 1 && (c.k_scale_stride[i] > kMaxIndex || c.v_scale_stride[i] > kMaxIndex)) return DSA_KV_ERR_UNSUPPORTED;
+  const int nb = a->G <= 8 ? 1 : 2;
+  const int64_t MT = ceil_div(a->G, 8 * nb);
   if (!fits(a->B, a->Q, c.H) || !fits(a->B * a->Q * c.H, MT, 1) || !fits(c.H, a->G, 1)) return DSA_KV_ERR_UNSUPPORTED;
   if (a->B == 0 || a->Q == 0) return DSA_KV_OK;
   if ((st = check_dense(a->q, a->B, a->Q, c.H * a->G, false)) != DSA_KV_OK) return st;
@@ -87,13 +98,42 @@ int attn(const dsa_kv_attn_args_t* a, void* stream) {
       !aligned(a->lse, 4))
     return DSA_KV_ERR_ALIGNMENT;
 
-  // Chunks: a block of more than 16 tokens is cut into pieces of 32, shorter
-  // blocks share a chunk by two (9 to 16 tokens) or four (8).
-  const int log_pieces = c.block_size > 16 ? 0 : c.block_size > 8 ? 1 : 2;
-  const int64_t per_block = log_pieces ? 1 : ceil_div(c.block_size, kTok);
+  const int64_t tiles = a->B * a->Q * c.H * MT;
+  const bool e = c.code_dtype == DSA_KV_E4M3, bf = a->dtype == DSA_KV_BF16;
+  const Variant v = bf ? (e ? variant_of<__nv_bfloat16, true>(c.D, nb) : variant_of<__nv_bfloat16, false>(c.D, nb))
+                       : (e ? variant_of<__half, true>(c.D, nb) : variant_of<__half, false>(c.D, nb));
+
+  // Chunks: a block of more than half a chunk is cut into chunks, shorter ones
+  // share a chunk, at most 8 of them (block_size >= 8).
+  int log_pieces = 0;
+  while ((v.tok >> (log_pieces + 1)) >= c.block_size) ++log_pieces;
+  const int piece = v.tok >> log_pieces;  // rows of a chunk for each block
+  const int64_t per_block = ceil_div(c.block_size, piece);
   const int64_t items = log_pieces ? ceil_div(a->K, 1 << log_pieces) : a->K * per_block;
   if (a->K > (1 << 30) || items > (1 << 30)) return DSA_KV_ERR_UNSUPPORTED;
-  const int box_rows = (int)(c.block_size < (kTok >> log_pieces) ? c.block_size : (kTok >> log_pieces));
+  const int box_rows = (int)(c.block_size < piece ? c.block_size : piece);
+
+  int dev;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return DSA_KV_ERR_CUDA;
+  int sms = g_sm_count[dev].load(std::memory_order_relaxed);
+  if (sms <= 0) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return DSA_KV_ERR_CUDA;
+    g_sm_count[dev].store(sms, std::memory_order_relaxed);
+  }
+  std::atomic<bool>& granted = g_granted[dev][(c.D / 128) * 8 + (nb - 1) * 4 + (e ? 2 : 0) + (bf ? 1 : 0)];
+  if (!granted.load(std::memory_order_relaxed)) {
+    if (cudaFuncSetAttribute(reinterpret_cast<const void*>(v.fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)(v.smem + (kMaxCluster - 1) * v.more)) != cudaSuccess)
+      return DSA_KV_ERR_CUDA;
+    granted.store(true, std::memory_order_relaxed);
+  }
+  // Few tiles: as many CTAs to each as stay resident at once, as long as every
+  // warp has a chunk. Measured (us with 1 / 2 / 4 / 8 CTAs per tile): 8 tiles of
+  // 32 chunks 15.6 / 11.3 / 9.4 / 8.9, 128 tiles of 64 chunks 34.4 / 27.2 / 32 /
+  // 43, 256 tiles of 128 chunks 91.5 / 96.3 / 105 / 136 (two CTAs fit an SM).
+  const int64_t resident = (int64_t)sms * v.ctas;
+  int cluster = 1;
+  while (cluster < kMaxCluster && tiles * cluster * 2 <= resident && items >= (int64_t)cluster * 2 * kAttnWarps) cluster *= 2;
 
   AttnParams p;
   p.q = dense(a->q);
@@ -101,8 +141,8 @@ int attn(const dsa_kv_attn_args_t* a, void* stream) {
   p.lse = a->lse;
   p.k_scale = c.k_scale;
   p.v_scale = c.v_scale;
-  p.ksp = c.k_scale_stride[0]; p.ksh = c.k_scale_stride[1]; p.kst = c.k_scale_stride[2];
-  p.vsp = c.v_scale_stride[0]; p.vsh = c.v_scale_stride[1]; p.vst = c.v_scale_stride[2];
+  p.ksp = (uint32_t)c.k_scale_stride[0]; p.ksh = (uint32_t)c.k_scale_stride[1]; p.kst = (uint32_t)c.k_scale_stride[2];
+  p.vsp = (uint32_t)c.v_scale_stride[0]; p.vsh = (uint32_t)c.v_scale_stride[1]; p.vst = (uint32_t)c.v_scale_stride[2];
   p.blocks = a->blocks;
   p.pages = a->pages;
   p.bsb = a->blocks_stride[0]; p.bsh = a->blocks_stride[1]; p.bsq = a->blocks_stride[2];
@@ -118,6 +158,8 @@ int attn(const dsa_kv_attn_args_t* a, void* stream) {
   p.G = (int32_t)a->G;
   p.K = (int32_t)a->K;
   p.bs = (int32_t)c.block_size;
+  p.cluster = (uint32_t)cluster;
+  p.early = tiles * cluster * 2 <= resident;
   p.log_pieces = log_pieces;
   p.box_bytes = (uint32_t)(box_rows * (c.D == 64 ? 64 : 128));
   p.block_bytes = bb;
@@ -129,19 +171,7 @@ int attn(const dsa_kv_attn_args_t* a, void* stream) {
                   !make_map(&v_map, c, c.v_codes, c.v_stride, box_rows)))
     return DSA_KV_ERR_CUDA;
 
-  const bool e = c.code_dtype == DSA_KV_E4M3, bf = a->dtype == DSA_KV_BF16;
-  const Variant v = bf ? (e ? variant_of<__nv_bfloat16, true>(c.D) : variant_of<__nv_bfloat16, false>(c.D))
-                       : (e ? variant_of<__half, true>(c.D) : variant_of<__half, false>(c.D));
-  int dev;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return DSA_KV_ERR_CUDA;
-  std::atomic<bool>& granted = g_granted[dev][(c.D / 128) * 4 + (e ? 2 : 0) + (bf ? 1 : 0)];
-  if (!granted.load(std::memory_order_relaxed)) {
-    if (cudaFuncSetAttribute(reinterpret_cast<const void*>(v.fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)v.smem) != cudaSuccess)
-      return DSA_KV_ERR_CUDA;
-    granted.store(true, std::memory_order_relaxed);
-  }
-  return launch(v.fn, a->B * a->Q * c.H * MT, kAttnWarps * 32, v.smem, stream, p, k_map, v_map);
+  return launch(v.fn, tiles * cluster, kAttnThreads, v.smem + (cluster - 1) * v.more, cluster, stream, p, k_map, v_map);
 }
 
 }  // namespace kv

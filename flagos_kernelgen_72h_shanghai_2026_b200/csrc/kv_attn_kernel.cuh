@@ -1,11 +1,13 @@
 // kv_attn_kernel.cuh — attention of query rows over selected blocks of the
 // quantised paged cache (dsa_kv_attn_launch, include/dsa_kv.h).
 //
-// A row (b, h, q) has G query heads that share a key head and a selection.
-// Up to 16 of them are the rows of one m16n8k16 tensor-core tile, on which a
-// CTA works. The row's selected tokens are cut into chunks of 32, dealt to the
-// warps in turn; every warp runs the one-pass softmax on its own chunks and
-// the partial results are joined at the end through shared memory.
+// A row (b, h, q) has G query heads that share a key head and a selection. A
+// CTA, or where there are few rows a cluster of up to 8 CTAs, works on 8 * NB
+// of them (NB = 1 or 2). The row's selected tokens are cut into chunks of TOK
+// = 32 or 64, dealt to the warps in turn; every warp runs the one-pass softmax on its own
+// chunks and the partial results are joined at the end through the cluster's
+// distributed shared memory: no workspace, no atomics, an order of summation
+// that does not vary.
 //
 // Mathematics, per query head, tokens t with key codes k, value codes v and
 // their scales ks, vs:
@@ -16,21 +18,30 @@
 // the weight of a token is at most 1 whatever the scales are, the products
 // run on raw codes (exact in fp16), and the maximum bounds each term of o.
 //
-// Precision: q is brought to fp16 by one power of two for the whole tile, its
+// Precision: q is brought to fp16 by one power of two for all heads of a CTA, the
 // largest value in [2^14, 2^15): bf16 values lose bits only 2^-28 below it.
 // Weights are fp16 too, times 2^6: 2^-11 relative (the output's own half step
 // is 2^-9 or 2^-12) down to 2^-20, with an absolute 2^-31 below. M lags behind
 // the maximum by up to 8 (a weight is at most 2^14), so that o is rescaled
 // only when the maximum really moves. Sums are fp32 throughout.
 //
-// Data movement: a chunk's key rows and value rows come by one TMA copy each
-// into a slot of the warp's own ring of S slots, so that no CTA barrier is
-// needed on the way and S - 1 chunks per warp stay in flight. Rows are 128
-// bytes (64 for D = 64), swizzled by the copy, which makes the 16-byte fragment
-// reads free of bank conflicts: lane (g, c) of a warp reads 32 contiguous
-// bytes of key row g for the products over D, whose order of summation is free
-// to choose, and 16 bytes of value rows 2c, 2c+1, 2c+8, 2c+9 for the products
-// over tokens, which are transposed pair by pair with byte permutes.
+// Tensor-core tiles (m16n8k16): tokens, then values of D, are the 16 rows and
+// query heads the 8 columns. Scores S = K q^T take 16 tokens x 8 heads at a
+// time, outputs O^T = V^T P^T 16 values of D x 8 heads. With heads as rows
+// instead, groups of up to 8 heads left half of every tile, and of the
+// exponentials and the output's registers, empty.
+//
+// Data movement: a chunk's key rows and value rows come by one TMA box each. A
+// warp has a ring of three boxes of its own, so that no CTA barrier is needed on
+// the way: the keys' box is refilled with the next chunk's values as soon as the
+// scores are done, the values' box with the keys of the chunk after that. Scales
+// follow by 4-byte asynchronous copies, and are turned into the token's factors
+// one chunk ahead. Rows are 128 bytes (64 for D = 64), swizzled by the copy,
+// which makes the 16-byte fragment reads free of bank conflicts: lane (g, c) of
+// a warp reads 32 contiguous bytes of key rows g and g + 8 for the products over
+// D, whose order of summation is free to choose, and 16 bytes of value rows 2c,
+// 2c+1, 2c+8, 2c+9 for the products over tokens, which are transposed pair by
+// pair with byte permutes. The weights change sides with movmatrix.
 #pragma once
 
 #include <cuda.h>
@@ -40,9 +51,9 @@
 
 namespace kv {
 
-constexpr int kTok = 32;           // tokens of a chunk
-constexpr int kRows = 16;          // query heads of a tile
 constexpr int kAttnWarps = 4;      // warps of a CTA
+constexpr int kAttnThreads = 32 * kAttnWarps;
+constexpr int kMaxCluster = 8;
 constexpr float kLift = 6.0f;      // weights are 2^(a - M + kLift)
 constexpr float kLag = 8.0f;       // M is moved when a maximum exceeds it by more
 constexpr uint64_t kAttnWaitNs = 2000000000ull;
@@ -52,37 +63,44 @@ struct AttnParams {
   float* lse;  // may be null
   const float* k_scale;
   const float* v_scale;
-  int64_t ksp, ksh, kst, vsp, vsh, vst;  // scale strides (page, head, token)
+  uint32_t ksp, ksh, kst, vsp, vsh, vst;  // scale strides (page, head, token)
   const void* blocks;
   const void* pages;
   int64_t bsb, bsh, bsq, psb, psh, psq;  // strides of blocks and pages (b, h, q)
   const void* q_pos;
   const void* kv_lens;
-  FastDiv MT, Q, H;     // tiles of 16 query heads per row, rows
+  FastDiv MT, Q, H;     // groups of 8 * NB query heads per row, rows
   FastDiv per_block;    // chunks of a block
   int64_t P;
   uint32_t items;       // chunks of a row
   int32_t G, K, bs;
-  int32_t log_pieces;   // a chunk holds 2^log_pieces blocks (blocks of at most 16 tokens)
+  int32_t log_pieces;   // a chunk holds 2^log_pieces blocks, where they are short
   uint32_t box_bytes;   // bytes of one copied box
   int32_t block_bytes, page_bytes, pos_bytes;
+  uint32_t cluster;     // CTAs that share a row's tokens
+  bool early;           // the next launch fits beside this one
   float scale;          // softmax_scale * log2(e)
 };
 
 // Shared-memory carve-up, identical on host and device.
-template <int D, int S>
+template <int D, int NB, int TOK>
 struct AttnSmem {
   static constexpr int W = kAttnWarps;
-  static constexpr size_t side = (size_t)kTok * D;  // one side of a slot
+  static constexpr int R = 8 * NB;                // query heads
+  static constexpr size_t box = (size_t)TOK * D;  // keys or values of a chunk
   static constexpr size_t ring = 0;
-  static constexpr size_t scales = ring + (size_t)W * S * 2 * side;
-  static constexpr size_t tok = scales + (size_t)W * S * 2 * kTok * 4;
-  static constexpr size_t flag = tok + (size_t)W * 3 * kTok * 4;
-  static constexpr size_t bars = flag + (size_t)W * S * kTok * 4;
-  static constexpr size_t ml = bars + (size_t)W * S * 8;        // [W][2][16] maxima and sums, then weights
-  static constexpr size_t fin = ml + (size_t)W * 2 * kRows * 4;  // [16] 1 / l
-  static constexpr size_t qf = fin + kRows * 4;
-  static constexpr size_t total = qf + (D == 256 ? (size_t)(D / 16) * 32 * 16 : 0);
+  static constexpr size_t region = 3 * box;       // of a warp; at the end its partial result
+  static_assert((size_t)R * D * 4 <= region, "the ring holds the partial result");
+  static constexpr size_t tok = ring + W * region;                   // [W][2][TOK] factors of a chunk's tokens
+  static constexpr size_t scales = tok + (size_t)W * 2 * TOK * 16;   // [W][2][2][TOK]
+  static constexpr size_t bars = scales + (size_t)W * 2 * 2 * TOK * 4;  // [W][3]
+  static constexpr size_t ml = bars + (size_t)W * 3 * 8;             // [W][2][R] maxima and sums
+  static constexpr size_t fin = ml + (size_t)W * 2 * R * 4;          // [R] 1 / l
+  static constexpr bool q_in_smem = D == 256 && NB == 2;             // where the output fills the registers
+  static constexpr size_t qf = fin + R * 4;
+  static constexpr size_t all = qf + (q_in_smem ? (size_t)(D / 16) * NB * 32 * 8 : 0);
+  // [C * W][2][R] of the cluster, then weights
+  static constexpr size_t total(int cluster) { return all + (size_t)cluster * W * 2 * R * 4; }
 };
 
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int tok, int head, int page,
@@ -93,22 +111,9 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
       "l"(map), "r"(x), "r"(tok), "r"(head), "r"(page), "r"(bar)
       : "memory");
 }
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(a)
-               : "memory");
-  return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
-  return v;
-}
 // c += a * b for one m16n8k16 tile, fp16 operands, fp32 sums.
 __device__ __forceinline__ void mma16816(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9},"
       " {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -119,14 +124,28 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The transposed 8 x 8 tile of 16-bit values.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 // Four codes -> two pairs of fp16 values (bytes 0, 1 and bytes 2, 3).
 // int8: the byte with its sign flipped, under the exponent of 1024, is the
 // fp16 number 1024 + 128 + code; both steps are exact.
 template <bool E4M3>
 __device__ __forceinline__ void decode_pairs(uint32_t w, uint32_t& lo, uint32_t& hi) {
   if (E4M3) {
-    lo = e4m3x2_to_half2((uint16_t)w);
-    hi = e4m3x2_to_half2((uint16_t)(w >> 16));
+    // one instruction each: the register's halves are named, not shifted
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
   } else {
     const uint32_t s = w ^ 0x80808080u, bias = 0x64806480u;
     const uint32_t a = __byte_perm(s, 0x64646464u, 0x4140), b = __byte_perm(s, 0x64646464u, 0x4342);
@@ -137,333 +156,471 @@ __device__ __forceinline__ void decode_pairs(uint32_t w, uint32_t& lo, uint32_t&
   }
 }
 
-// Place of float4 `f4` of row `row` in a warp's partial result: the units of a
-// row are permuted so that the writes of a quarter warp spread over the banks.
-template <int D>
-__device__ __forceinline__ int part_index(int row, int f4) {
-  const int c = D == 64 ? (f4 >> 2) & 3 : (f4 >> 3) & 3;
-  return row * (D / 4) + (f4 ^ ((c * 2 + (row & 1)) & 7));
+// Address of another CTA's shared memory in the cluster, and loads from it.
+__device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
-template <typename T, int D, bool E4M3, int S>
-__global__ void __launch_bounds__(kAttnWarps * 32)
+// Place of float4 `f4` of head `row` in a warp's partial result: the units of a
+// head are permuted so that the writes of a quarter warp spread over the banks.
+template <int D>
+__device__ __forceinline__ int part_index(int row, int f4) {
+  const int c = (row >> 1) & 3;
+  return row * (D / 4) + (f4 ^ (D == 64 ? (c & 1) | ((c >> 1) << 2) : c));
+}
+
+template <typename T, int D, bool E4M3, int NB, int TOK, int CTAS>
+__global__ void __launch_bounds__(kAttnThreads, CTAS)
     attn_kernel(const AttnParams p, const __grid_constant__ CUtensorMap k_map,
                 const __grid_constant__ CUtensorMap v_map) {
-  using L = AttnSmem<D, S>;
-  constexpr int W = kAttnWarps;
-  constexpr int NH = D == 256 ? 2 : 1;    // boxes of at most 128 bytes per side
+  using L = AttnSmem<D, NB, TOK>;
+  constexpr int W = kAttnWarps, R = L::R;
+  constexpr int NH = D == 256 ? 2 : 1;    // boxes of at most 128 bytes' width per side
   constexpr int NU = D == 64 ? 1 : 2;     // 16-byte pieces of a key row per lane and box
-  constexpr int NT = D / 8;               // 8-wide column tiles of the output
+  constexpr int NT = D / 16;              // 16-row tiles of the output
+  constexpr int NS = TOK / 16;            // 16-row tiles of the scores
+  constexpr int LT = TOK / 32;            // tokens of a lane, where each token has one: lane, lane + 32
+  constexpr int LOG_TOK = TOK == 64 ? 6 : 5;
   constexpr int ROWB = D == 64 ? 64 : 128;
-  constexpr bool QSMEM = D == 256;        // q fragments in shared memory (registers hold the output)
+  constexpr bool QSMEM = L::q_in_smem;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  uint32_t r = blockIdx.x, mt, qi, h, b;
+  const uint32_t C = p.cluster, rank = blockIdx.x & (C - 1), NW = C * W, wid = rank * W + warp;
+  uint32_t r = blockIdx.x / C, mt, qi, h, b;
   p.MT.divmod(r, &r, &mt);
   p.Q.divmod(r, &r, &qi);
   p.H.divmod(r, &b, &h);
-  const int head0 = (int)h * p.G + (int)mt * kRows;
-  const int rows = min(kRows, p.G - (int)mt * kRows);
+  const int head0 = (int)h * p.G + (int)mt * R;
+  const int rows = min(R, p.G - (int)mt * R);
 
   const uint32_t base = farq::smem_u32(smem);
-  const uint32_t slots = base + (uint32_t)L::ring + warp * (uint32_t)(S * 2 * L::side);
-  const uint32_t bars = base + (uint32_t)L::bars + warp * S * 8;
-  float* const scales = reinterpret_cast<float*>(smem + L::scales) + warp * S * 2 * kTok;
-  float* const tok = reinterpret_cast<float*>(smem + L::tok) + warp * 3 * kTok;
-  uint32_t* const flags = reinterpret_cast<uint32_t*>(smem + L::flag) + warp * S * kTok;
+  uint8_t* const ring = smem + L::ring + warp * L::region;
+  const uint32_t bars = base + (uint32_t)L::bars + warp * 3 * 8;
+  float* const scales = reinterpret_cast<float*>(smem + L::scales) + warp * 2 * 2 * TOK;
+  float4* const tok = reinterpret_cast<float4*>(smem + L::tok) + warp * 2 * TOK;
   if (lane == 0) {
-    for (int s = 0; s < S; ++s) farq::mbar_init(bars + 8 * s, 1);
+    for (int s = 0; s < 3; ++s) farq::mbar_init(bars + 8 * s, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
   }
   __syncwarp();
-  pdl_wait();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // The next launch may come in: at once where it finds room beside this one,
+  // else when this one's CTAs are about to end. Earlier, its waiting CTAs would
+  // take the places that this grid's last CTAs need to spread evenly.
+  if (p.early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // Tokens t < lim count: the causal limit and the sequence's length.
+  // Everything the first copies depend on is loaded at once: position and
+  // length, the first 32 pieces of the selection, the queries.
   const int64_t pos = load_index(p.q_pos, (int64_t)b * p.Q.d + qi, p.pos_bytes);
   int64_t lim = load_index(p.kv_lens, b, p.pos_bytes);
-  if (pos < lim) lim = pos + 1;
-  if (pos < 0) lim = 0;
-  lim = min(lim, (int64_t)1 << 40);  // so that no product below overflows
-  const uint32_t items = lim > 0 ? p.items : 0;
-  const uint32_t NW = W, wid = warp;
   const int64_t brow = b * p.bsb + h * p.bsh + qi * p.bsq;
   const int64_t prow = b * p.psb + h * p.psh + qi * p.psq;
+  const float* const k_scale = p.k_scale + (uint64_t)h * p.ksh;
+  const float* const v_scale = p.v_scale + (uint64_t)h * p.vsh;
 
-  // The warp looks its chunks up 32 pieces at a time; a lane holds one piece:
-  // page, first token within the page, valid tokens.
-  const int lp = p.log_pieces, pitch = kTok >> lp;
-  uint32_t next_k = 0, active = 0;
+  // The warp looks its chunks up 32 pieces at a time (with lp = 0 a chunk is
+  // one piece); a lane holds one: page, first token within the page, tokens
+  // that count.
+  const int lp = p.log_pieces, per = 1 << lp, pitch = TOK >> lp;
+  uint32_t next_k = 0, active = 0, pieces = 0;  // chunks and pieces of this look-up that are left
   int pc_page = 0, pc_off = 0, pc_n = 0;
-  auto look_up = [&] {
+  int64_t ld_blk, ld_page;
+  uint32_t ld_sub;
+  auto fetch = [&] {  // the next 32 pieces' entries
     const uint32_t item = wid + (next_k + (lane >> lp)) * NW;
     next_k += 32 >> lp;
-    uint32_t entry, sub = 0;
+    uint32_t entry;
+    ld_sub = 0;
     if (lp == 0)
-      p.per_block.divmod(item, &entry, &sub);
+      p.per_block.divmod(item, &entry, &ld_sub);
     else
-      entry = (item << lp) + (lane & ((1 << lp) - 1));
-    pc_n = 0;
-    if (item < items && entry < (uint32_t)p.K) {
-      const int64_t blk = load_index(p.blocks, brow + entry, p.block_bytes);
-      const int64_t page = load_index(p.pages, prow + entry, p.page_bytes);
-      if (blk >= 0 && blk < lim && page >= 0 && page < p.P) {
-        const int64_t left = lim - (blk * p.bs + (int64_t)sub * kTok);
-        const int most = min(kTok, p.bs - (int)sub * kTok);
-        pc_n = left <= 0 ? 0 : left < most ? (int)left : most;
-        pc_page = (int)page;
-        pc_off = (int)sub * kTok;
-      }
+      entry = (item << lp) + (lane & (per - 1));
+    ld_blk = ld_page = -1;
+    if (item < p.items && entry < (uint32_t)p.K) {
+      ld_blk = load_index(p.blocks, brow + entry, p.block_bytes);
+      ld_page = load_index(p.pages, prow + entry, p.page_bytes);
     }
-    active = __ballot_sync(0xffffffffu, pc_n > 0);
+  };
+  auto look_up = [&] {
+    pc_n = 0;
+    if (ld_blk >= 0 && ld_blk < lim && ld_page >= 0 && ld_page < p.P) {
+      const int64_t left = lim - (ld_blk * p.bs + (int64_t)ld_sub * TOK);
+      const int most = min(TOK, p.bs - (int)ld_sub * TOK);
+      pc_n = left <= 0 ? 0 : left < most ? (int)left : most;
+      pc_page = (int)ld_page;
+      pc_off = (int)ld_sub * TOK;
+    }
+    active = pieces = __ballot_sync(0xffffffffu, pc_n > 0);
     if (lp >= 1) active |= active >> 1;
     if (lp >= 2) active |= active >> 2;
-    if (lp >= 1) active &= lp == 1 ? 0x55555555u : 0x11111111u;
+    if (lp >= 3) active |= active >> 4;
+    if (lp >= 1) active &= lp == 1 ? 0x55555555u : lp == 2 ? 0x11111111u : 0x01010101u;
   };
-  // Starts the copies of the warp's next chunk into a slot; false when there is none.
-  auto issue = [&](int s) -> bool {
+  // The chunk whose keys, and then values, are copied next: the piece that
+  // this lane copies (lanes 0 to 2^lp - 1), its tokens and their scales.
+  bool more = true;
+  int cp_page = 0, cp_off = 0;
+  bool copies = false;
+  uint32_t cp_bytes = 0, cp_mask[LT];
+  const float *cp_ks[LT], *cp_vs[LT];
+  auto prepare = [&] {
     while (active == 0) {
-      if (wid + next_k * NW >= items) return false;
+      if (wid + next_k * NW >= p.items) {
+        more = false;
+        return;
+      }
+      fetch();
       look_up();
     }
     const int first = __ffs(active) - 1;
     active &= active - 1;
-    // scales, and whether the token counts, of this lane's token
-    const int src = first + (lane >> (5 - lp)), j = lane & (pitch - 1);
-    const int64_t page = __shfl_sync(0xffffffffu, pc_page, src);
-    const int64_t at = __shfl_sync(0xffffffffu, pc_off, src) + j;
-    const bool valid = j < __shfl_sync(0xffffffffu, pc_n, src);
-    const float* ks = p.k_scale;
-    const float* vs = p.v_scale;
-    if (valid) {
-      ks += page * p.ksp + h * p.ksh + at * p.kst;
-      vs += page * p.vsp + h * p.vsh + at * p.vst;
+    const uint32_t here = (pieces >> first) & ((1u << per) - 1);
+    cp_bytes = __popc(here) * NH * p.box_bytes;
+    copies = lane < per && ((here >> lane) & 1);
+#pragma unroll
+    for (int t = 0; t < LT; ++t) {
+      const int src = first + ((lane + 32 * t) >> (LOG_TOK - lp)), j = (lane + 32 * t) & (pitch - 1);
+      const uint32_t page = __shfl_sync(0xffffffffu, pc_page, src);
+      const uint32_t at = __shfl_sync(0xffffffffu, pc_off, src) + j;
+      cp_mask[t] = __ballot_sync(0xffffffffu, j < __shfl_sync(0xffffffffu, pc_n, src));
+      cp_ks[t] = k_scale + (uint64_t)page * p.ksp + (uint64_t)at * p.kst;
+      cp_vs[t] = v_scale + (uint64_t)page * p.vsp + (uint64_t)at * p.vst;
     }
-    const uint32_t sdst = farq::smem_u32(scales + s * 2 * kTok + lane), bytes = valid ? 4 : 0;
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(sdst), "l"(ks), "r"(bytes) : "memory");
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(sdst + kTok * 4), "l"(vs), "r"(bytes) : "memory");
-    flags[s * kTok + lane] = valid;
-    // one copy per piece and box, by the lane that holds the piece
-    const int piece = lane - first;
-    const bool copies = piece >= 0 && piece < (1 << lp) && pc_n > 0;
-    const uint32_t n = __popc(__ballot_sync(0xffffffffu, copies));
+    cp_page = __shfl_sync(0xffffffffu, pc_page, first + lane);
+    cp_off = __shfl_sync(0xffffffffu, pc_off, first + lane);
+  };
+  auto copy = [&](const CUtensorMap* map, int s) {
     const uint32_t bar = bars + 8 * s;
-    if (lane == first) farq::mbar_arrive_expect_tx(bar, n * 2 * NH * p.box_bytes);
+    if (lane == 0) farq::mbar_arrive_expect_tx(bar, cp_bytes);
     __syncwarp();
     if (copies) {
-      const uint32_t dst = slots + s * (uint32_t)(2 * L::side) + piece * pitch * ROWB;
+      const uint32_t dst = farq::smem_u32(ring) + s * (uint32_t)L::box + lane * pitch * ROWB;
 #pragma unroll
-      for (int hh = 0; hh < NH; ++hh) {
-        tma_load(dst + hh * kTok * 128, &k_map, hh * 128, pc_off, h, pc_page, bar);
-        tma_load(dst + (uint32_t)L::side + hh * kTok * 128, &v_map, hh * 128, pc_off, h, pc_page, bar);
-      }
+      for (int hh = 0; hh < NH; ++hh) tma_load(dst + hh * TOK * 128, map, hh * 128, cp_off, h, cp_page, bar);
     }
-    return true;
   };
-
-  uint32_t issued = 0;
-  bool more = true;
+  // Scales of this lane's tokens; zeros, and no access, where there are none.
+  auto copy_scales = [&](int buf) {
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
-    if (more && (more = issue(s))) ++issued;
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    for (int t = 0; t < LT; ++t) {
+      const bool valid = (cp_mask[t] >> lane) & 1;
+      const uint32_t dst = farq::smem_u32(scales + buf * 2 * TOK + 32 * t + lane), bytes = valid ? 4 : 0;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(valid ? cp_ks[t] : k_scale), "r"(bytes)
+                   : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + TOK * 4), "l"(valid ? cp_vs[t] : v_scale),
+                   "r"(bytes)
+                   : "memory");
+    }
+  };
+  // Factors of this lane's tokens: of their scores, the exponent and the
+  // inverse of their value scales.
+  auto factors = [&](int buf) {
+#pragma unroll
+    for (int t = 0; t < LT; ++t) {
+      const float ks = scales[buf * 2 * TOK + 32 * t + lane];
+      float vs = scales[buf * 2 * TOK + TOK + 32 * t + lane];
+      vs = vs < kMinScale ? kMinScale : vs;
+      tok[buf * TOK + 32 * t + lane] = make_float4(ks * p.scale, __log2f(vs), rcp_approx(vs), 0.f);
+    }
+  };
+  // Rows that hold no token of the row: whatever lies there becomes zeros.
+  auto clear = [&](uint8_t* box, const uint32_t (&mask)[LT]) {
+    bool partial = false;
+#pragma unroll
+    for (int t = 0; t < LT; ++t) partial |= mask[t] != 0xffffffffu;
+    if (!partial) return;
+#pragma unroll
+    for (int t = 0; t < LT; ++t)
+      if (!((mask[t] >> lane) & 1)) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+          *reinterpret_cast<uint4*>(box + (i / 8) * TOK * 128 + (lane + 32 * t) * ROWB + (i % 8) * 16) =
+              make_uint4(0, 0, 0, 0);
+      }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+  };
+  fetch();
+
+  // Queries: lane (g, c) holds heads g, g + 8, values 32c + 16u + 4i .. + 3 of
+  // each box (16c + 4i .. + 3 where D = 64), in the order of its key bytes.
+  uint4 raw[NB][NH][NU * 2];
+#pragma unroll
+  for (int x = 0; x < NB; ++x) {
+    const bool in = g + 8 * x < rows;
+    const uint8_t* src = p.q.row(b, qi, head0 + (in ? g + 8 * x : 0)) + c * (NU * 32);
+#pragma unroll
+    for (int hh = 0; hh < NH; ++hh)
+#pragma unroll
+      for (int i = 0; i < NU * 2; ++i) raw[x][hh][i] = in ? ld_stream(src + hh * 256 + i * 16) : make_uint4(0, 0, 0, 0);
   }
 
-  // The tile's q in fp16, as fragments of 16 values of D at a time: lane
-  // (g, c) holds rows g and g + 8, values 32c + 16u + 4i .. + 3 of each box
-  // (16c + 4i .. + 3 where D = 64), in the order of its key bytes.
-  uint32_t qf[QSMEM ? 1 : D / 16][4];
+  // Tokens t < lim count: the causal limit and the sequence's length.
+  if (pos < lim) lim = pos + 1;
+  if (pos < 0) lim = 0;
+  lim = min(lim, (int64_t)1 << 40);  // so that no product overflows
+  look_up();
+  // The first chunk, and the second one's keys.
+  uint32_t issued = 0, mask[LT], next_mask[LT];
+#pragma unroll
+  for (int t = 0; t < LT; ++t) mask[t] = next_mask[t] = 0;
+  more = lim > 0;
+  if (more) prepare();
+  if (more) {
+    copy(&k_map, 0);
+    copy_scales(0);
+    copy(&v_map, 1);
+    ++issued;
+#pragma unroll
+    for (int t = 0; t < LT; ++t) mask[t] = cp_mask[t];
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  if (more) prepare();
+  if (more) {
+    copy(&k_map, 2);
+    copy_scales(1);
+    ++issued;
+#pragma unroll
+    for (int t = 0; t < LT; ++t) next_mask[t] = cp_mask[t];
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+
+  // In fp16, times the power of two that brings the CTA's largest finite value
+  // into [2^14, 2^15).
+  uint32_t qf[QSMEM ? 1 : D / 16][NB][2];
   float qs;
   {
-    uint4 raw[2][NH][NU * 2];
     float most = 0.f;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const bool in = g + 8 * x < rows;
-      const uint8_t* src = p.q.row(b, qi, head0 + (in ? g + 8 * x : 0)) + c * (NU * 32);
+    for (int x = 0; x < NB; ++x)
 #pragma unroll
       for (int hh = 0; hh < NH; ++hh)
 #pragma unroll
         for (int i = 0; i < NU * 2; ++i) {
-          raw[x][hh][i] = in ? ld_stream(src + hh * 256 + i * 16) : make_uint4(0, 0, 0, 0);
           float f[8];
           unpack8<T>(raw[x][hh][i], f);
 #pragma unroll
           for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[e]) <= 3.4e38f ? fabsf(f[e]) : 0.f);
         }
-    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    // the power of two that brings the largest finite value into [2^14, 2^15)
     const int ex = max((int)(__float_as_uint(most) >> 23) - 127, -100);
     const float up = most > 0.f ? __uint_as_float((uint32_t)(14 - ex + 127) << 23) : 1.f;
-    qs = p.scale / up;
+    qs = 1.f / up;
 #pragma unroll
-    for (int hh = 0; hh < NH; ++hh)
+    for (int x = 0; x < NB; ++x)
 #pragma unroll
-      for (int i = 0; i < NU * 2; ++i) {
-        uint32_t w[2][4];
+      for (int hh = 0; hh < NH; ++hh)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
+        for (int i = 0; i < NU * 2; ++i) {
           float f[8];
           unpack8<T>(raw[x][hh][i], f);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[x][e] = Half16<__half>::pack(f[2 * e] * up, f[2 * e + 1] * up);
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int ks = (hh * NU * 2 + i) * 2 + e;
-          const uint32_t a[4] = {w[0][2 * e], w[1][2 * e], w[0][2 * e + 1], w[1][2 * e + 1]};
-          if (QSMEM) {
-            if (warp == 0)
-              *reinterpret_cast<uint4*>(smem + L::qf + (ks * 32 + lane) * 16) = make_uint4(a[0], a[1], a[2], a[3]);
-          } else {
-#pragma unroll
-            for (int y = 0; y < 4; ++y) qf[QSMEM ? 0 : ks][y] = a[y];
+          for (int e = 0; e < 2; ++e) {
+            const int ks = (hh * NU * 2 + i) * 2 + e;
+            const uint32_t b0 = Half16<__half>::pack(f[4 * e] * up, f[4 * e + 1] * up);
+            const uint32_t b1 = Half16<__half>::pack(f[4 * e + 2] * up, f[4 * e + 3] * up);
+            if (QSMEM) {
+              if (warp == 0) *reinterpret_cast<uint2*>(smem + L::qf + ((ks * NB + x) * 32 + lane) * 8) = make_uint2(b0, b1);
+            } else {
+              qf[QSMEM ? 0 : ks][x][0] = b0;
+              qf[QSMEM ? 0 : ks][x][1] = b1;
+            }
           }
         }
-      }
     if (QSMEM) __syncthreads();
   }
 
-  float o[NT][4];
+  float o[NT][NB][4];
+  float M[NB][2];  // of heads 2c, 2c + 1 (+ 8x)
+  f32x2 l[NB], from[NB];  // sums of weights; kLift - M
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
+  for (int x = 0; x < NB; ++x) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-  float M0 = -INFINITY, M1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][x][e] = 0.f;
+    M[x][0] = M[x][1] = -INFINITY;
+    l[x] = 0;
+    from[x] = pair(kLift, kLift);
+  }
   bool failed = false;
 
-  int s = 0;
-  uint32_t parity = 0;
+  int s = 0;            // box of this chunk's keys; its values are in the next one
+  uint32_t parity = 0;  // of that box's copy
+  asm volatile("cp.async.wait_group 1;" ::: "memory");
+  if (issued > 0) factors(0);
+  __syncwarp();
   for (uint32_t n = 0; n < issued; ++n) {
-    const uint32_t kslot = slots + s * (uint32_t)(2 * L::side), vslot = kslot + (uint32_t)L::side;
-    asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
-    // this lane's token: factor of its scores, exponent and inverse of its value scale
-    const uint32_t valid = flags[s * kTok + lane];
-    {
-      const float ks = scales[s * 2 * kTok + lane];
-      float vs = scales[s * 2 * kTok + kTok + lane];
-      vs = vs < kMinScale ? kMinScale : vs;
-      tok[lane] = ks * qs;
-      tok[kTok + lane] = __log2f(vs);
-      tok[2 * kTok + lane] = __frcp_rn(vs);
-    }
-    const uint32_t mask = __ballot_sync(0xffffffffu, valid != 0);
+    const float4* const now = tok + (n & 1) * TOK;
+    const int sv = s == 2 ? 0 : s + 1;
+    const uint32_t parity_v = s == 2 ? parity ^ 1 : parity;
+    uint8_t* const kbox = ring + s * L::box;
+    uint8_t* const vbox = ring + sv * L::box;
     if (!farq::mbar_wait_bounded(bars + 8 * s, parity, kAttnWaitNs)) failed = true;
     if (__any_sync(0xffffffffu, failed)) {
       failed = true;
       break;
     }
-    if (mask != 0xffffffffu) {
-      // rows that hold no token of the row: whatever lies there becomes zeros
-      if (!valid) {
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          const uint32_t at = (i / 8) * kTok * 128 + lane * ROWB + (i % 8) * 16;
-          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(kslot + at), "r"(0) : "memory");
-          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vslot + at), "r"(0) : "memory");
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      }
-    }
-    __syncwarp();
+    clear(kbox, mask);
 
-    // scores of 16 heads x 32 tokens
-    float sc[4][4];
+    // scores: tile t has tokens 16t + g and 16t + g + 8 as this lane's rows
+    float sc[NS][NB][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int t = 0; t < NS; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sc[j][e] = 0.f;
+      for (int x = 0; x < NB; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[t][x][e] = 0.f;
 #pragma unroll
     for (int hh = 0; hh < NH; ++hh)
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
-        uint4 kw[4];
+        uint4 kw[2 * NS];  // key rows 8j + g
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 2 * NS; ++j) {
           const uint32_t at = D == 64 ? (8 * j + g) * 64 + ((c ^ ((g >> 1) & 3)) << 4)
-                                      : hh * kTok * 128 + (8 * j + g) * 128 + (((2 * c + u) ^ g) << 4);
-          kw[j] = lds128(kslot + at);
+                                      : hh * TOK * 128 + (8 * j + g) * 128 + (((2 * c + u) ^ g) << 4);
+          kw[j] = *reinterpret_cast<const uint4*>(kbox + at);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int ks = (hh * NU + u) * 4 + i;
-          uint32_t a[4];
-          if (QSMEM) {
-            const uint4 t = lds128(base + (uint32_t)L::qf + (ks * 32 + lane) * 16);
-            a[0] = t.x; a[1] = t.y; a[2] = t.z; a[3] = t.w;
-          } else {
+          uint32_t bq[NB][2];
 #pragma unroll
-            for (int y = 0; y < 4; ++y) a[y] = qf[QSMEM ? 0 : ks][y];
+          for (int x = 0; x < NB; ++x) {
+            if (QSMEM) {
+              const uint2 v = *reinterpret_cast<const uint2*>(smem + L::qf + ((ks * NB + x) * 32 + lane) * 8);
+              bq[x][0] = v.x;
+              bq[x][1] = v.y;
+            } else {
+              bq[x][0] = qf[QSMEM ? 0 : ks][x][0];
+              bq[x][1] = qf[QSMEM ? 0 : ks][x][1];
+            }
           }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t w = i == 0 ? kw[j].x : i == 1 ? kw[j].y : i == 2 ? kw[j].z : kw[j].w;
-            uint32_t b0, b1;
-            decode_pairs<E4M3>(w, b0, b1);
-            mma16816(sc[j], a, b0, b1);
+          for (int t = 0; t < NS; ++t) {
+            const uint4 &lo = kw[2 * t], &hi = kw[2 * t + 1];
+            uint32_t a[4];
+            decode_pairs<E4M3>(i == 0 ? lo.x : i == 1 ? lo.y : i == 2 ? lo.z : lo.w, a[0], a[2]);
+            decode_pairs<E4M3>(i == 0 ? hi.x : i == 1 ? hi.y : i == 2 ? hi.z : hi.w, a[1], a[3]);
+#pragma unroll
+            for (int x = 0; x < NB; ++x) mma16816(sc[t][x], a, bq[x][0], bq[x][1]);
           }
         }
       }
+    __syncwarp();  // the keys are read
+    if (n + 1 < issued) copy(&v_map, s);
+    if (more) prepare();
 
-    // weights; columns 2c, 2c + 1 of tile j are tokens 8j + 2c, 8j + 2c + 1
-    float inv[4][2], m0 = -INFINITY, m1 = -INFINITY;
+    // exponents of heads 2c, 2c + 1 and tokens 8j + g. M moves when a lane
+    // sees a value well above it; until then nothing has to be exchanged
+    // between lanes.
+    f32x2 a[2 * NS][NB];
+    float inv[2 * NS], m[NB][2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = *reinterpret_cast<const float2*>(tok + 8 * j + 2 * c);
-      const float2 lv = *reinterpret_cast<const float2*>(tok + kTok + 8 * j + 2 * c);
-      const float2 iv = *reinterpret_cast<const float2*>(tok + 2 * kTok + 8 * j + 2 * c);
-      inv[j][0] = iv.x;
-      inv[j][1] = iv.y;
-      sc[j][0] = fmaf(sc[j][0], f.x, lv.x);
-      sc[j][1] = fmaf(sc[j][1], f.y, lv.y);
-      sc[j][2] = fmaf(sc[j][2], f.x, lv.x);
-      sc[j][3] = fmaf(sc[j][3], f.y, lv.y);
-      if (mask != 0xffffffffu) {
-        const uint32_t bits = mask >> (8 * j + 2 * c);
-        if (!(bits & 1)) sc[j][0] = sc[j][2] = -INFINITY;
-        if (!(bits & 2)) sc[j][1] = sc[j][3] = -INFINITY;
+    for (int x = 0; x < NB; ++x) m[x][0] = m[x][1] = -INFINITY;
+    bool partial = false;
+#pragma unroll
+    for (int t = 0; t < LT; ++t) partial |= mask[t] != 0xffffffffu;
+#pragma unroll
+    for (int j = 0; j < 2 * NS; ++j) {
+      const float4 f = now[8 * j + g];
+      const float fx = f.x * qs;
+      inv[j] = f.z;
+#pragma unroll
+      for (int x = 0; x < NB; ++x)
+        a[j][x] = fma2(pair(sc[j >> 1][x][(j & 1) * 2], sc[j >> 1][x][(j & 1) * 2 + 1]), pair(fx, fx), pair(f.y, f.y));
+    }
+    if (partial) {
+#pragma unroll
+      for (int j = 0; j < 2 * NS; ++j)
+#pragma unroll
+        for (int x = 0; x < NB; ++x)
+          if (!((mask[j / 4] >> (8 * (j & 3) + g)) & 1)) a[j][x] = pair(-INFINITY, -INFINITY);
+    }
+    bool moves = false;
+#pragma unroll
+    for (int x = 0; x < NB; ++x) {
+#pragma unroll
+      for (int j = 0; j < 2 * NS; ++j) {
+        const float2 v = both(a[j][x]);
+        m[x][0] = fmaxf(m[x][0], v.x);
+        m[x][1] = fmaxf(m[x][1], v.y);
       }
-      m0 = fmaxf(m0, fmaxf(sc[j][0], sc[j][1]));
-      m1 = fmaxf(m1, fmaxf(sc[j][2], sc[j][3]));
+      moves |= m[x][0] > M[x][0] + kLag || m[x][1] > M[x][1] + kLag;
     }
+    if (__any_sync(0xffffffffu, moves)) {
 #pragma unroll
-    for (int x = 1; x <= 2; x <<= 1) {
-      m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, x));
-      m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, x));
-    }
-    if (__any_sync(0xffffffffu, m0 > M0 + kLag || m1 > M1 + kLag)) {
-      const float n0 = fmaxf(M0, m0), n1 = fmaxf(M1, m1);
-      const float f0 = M0 == n0 ? 1.f : exp2_approx(M0 - n0), f1 = M1 == n1 ? 1.f : exp2_approx(M1 - n1);
-      M0 = n0;
-      M1 = n1;
-      l0 *= f0;
-      l1 *= f1;
+      for (int x = 0; x < NB; ++x) {
+        float f[2];
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        o[i][0] *= f0;
-        o[i][1] *= f0;
-        o[i][2] *= f1;
-        o[i][3] *= f1;
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int y = 4; y <= 16; y <<= 1) m[x][e] = fmaxf(m[x][e], __shfl_xor_sync(0xffffffffu, m[x][e], y));
+          const float top = fmaxf(M[x][e], m[x][e]);
+          f[e] = M[x][e] == top ? 1.f : exp2_approx(M[x][e] - top);
+          M[x][e] = top;
+        }
+        l[x] = mul2(l[x], pair(f[0], f[1]));
+        from[x] = pair(kLift - (M[x][0] == -INFINITY ? 0.f : M[x][0]), kLift - (M[x][1] == -INFINITY ? 0.f : M[x][1]));
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          o[i][x][0] *= f[0];
+          o[i][x][1] *= f[1];
+          o[i][x][2] *= f[0];
+          o[i][x][3] *= f[1];
+        }
       }
     }
-    const float s0 = kLift - (M0 == -INFINITY ? 0.f : M0), s1 = kLift - (M1 == -INFINITY ? 0.f : M1);
-    uint32_t pw[4][2];
+    // weights, as the columns of the second product: tokens 2c, 2c + 1 of head g
+    uint32_t pw[2 * NS][NB];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float w0 = exp2_approx(sc[j][0] + s0), w1 = exp2_approx(sc[j][1] + s0);
-      const float w2 = exp2_approx(sc[j][2] + s1), w3 = exp2_approx(sc[j][3] + s1);
-      l0 = fmaf(w0, inv[j][0], fmaf(w1, inv[j][1], l0));
-      l1 = fmaf(w2, inv[j][0], fmaf(w3, inv[j][1], l1));
-      pw[j][0] = Half16<__half>::pack(w0, w1);
-      pw[j][1] = Half16<__half>::pack(w2, w3);
-    }
+    for (int x = 0; x < NB; ++x)
+#pragma unroll
+      for (int j = 0; j < 2 * NS; ++j) {
+        const float2 e = both(add2(a[j][x], from[x]));
+        const float w0 = exp2_approx(e.x), w1 = exp2_approx(e.y);
+        l[x] = fma2(pair(w0, w1), pair(inv[j], inv[j]), l[x]);
+        pw[j][x] = transpose8x8(Half16<__half>::pack(w0, w1));
+      }
 
-    // weights times values; column g of output tile x is value 16g + x of its box (8g + x where D = 64)
+    // the next chunk's factors
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    factors((n & 1) ^ 1);
+
+    if (!farq::mbar_wait_bounded(bars + 8 * sv, parity_v, kAttnWaitNs)) failed = true;
+    if (__any_sync(0xffffffffu, failed)) {
+      failed = true;
+      break;
+    }
+    clear(vbox, mask);
+    // values times weights; rows g and g + 8 of output tile y are values
+    // 16g + 2y and 16g + 2y + 1 of their box (8g + .. where D = 64)
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint32_t a[4] = {pw[2 * t][0], pw[2 * t][1], pw[2 * t + 1][0], pw[2 * t + 1][1]};
+    for (int t = 0; t < NS; ++t) {
 #pragma unroll
       for (int hh = 0; hh < NH; ++hh) {
         constexpr int NWORD = D == 64 ? 2 : 4;
@@ -472,11 +629,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32)
         for (int x = 0; x < 4; ++x) {
           const int row = 16 * t + 2 * c + (x & 1) + 8 * (x >> 1);
           if constexpr (D == 64) {
-            const uint2 v = lds64(vslot + row * 64 + (((g >> 1) ^ c) << 4) + (g & 1) * 8);
+            const uint2 v = *reinterpret_cast<const uint2*>(vbox + row * 64 + (((g >> 1) ^ c) << 4) + (g & 1) * 8);
             w[x][0] = v.x;
             w[x][1] = v.y;
           } else {
-            const uint4 v = lds128(vslot + hh * kTok * 128 + row * 128 + ((g ^ (2 * c + (x & 1))) << 4));
+            const uint4 v = *reinterpret_cast<const uint4*>(vbox + hh * TOK * 128 + row * 128 + ((g ^ (2 * c + (x & 1))) << 4));
             w[x][0] = v.x;
             w[x][1] = v.y;
             w[x][2] = v.z;
@@ -484,99 +641,115 @@ __global__ void __launch_bounds__(kAttnWarps * 32)
           }
         }
 #pragma unroll
-        for (int i = 0; i < NWORD; ++i) {
-          uint32_t b0[4], b1[4];
-          decode_pairs<E4M3>(__byte_perm(w[0][i], w[1][i], 0x5140), b0[0], b0[1]);
-          decode_pairs<E4M3>(__byte_perm(w[0][i], w[1][i], 0x7362), b0[2], b0[3]);
-          decode_pairs<E4M3>(__byte_perm(w[2][i], w[3][i], 0x5140), b1[0], b1[1]);
-          decode_pairs<E4M3>(__byte_perm(w[2][i], w[3][i], 0x7362), b1[2], b1[3]);
+        for (int i = 0; i < NWORD; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mma16816(o[hh * 16 + 4 * i + e], a, b0[e], b1[e]);
-        }
+          for (int e = 0; e < 2; ++e) {
+            uint32_t a[4];
+            decode_pairs<E4M3>(__byte_perm(w[0][i], w[1][i], e ? 0x7362 : 0x5140), a[0], a[1]);
+            decode_pairs<E4M3>(__byte_perm(w[2][i], w[3][i], e ? 0x7362 : 0x5140), a[2], a[3]);
+#pragma unroll
+            for (int x = 0; x < NB; ++x) mma16816(o[hh * 8 + 2 * i + e][x], a, pw[2 * t][x], pw[2 * t + 1][x]);
+          }
       }
     }
-    __syncwarp();  // the slot and the token factors are read
-    if (more && (more = issue(s))) ++issued;
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    if (++s == S) {
-      s = 0;
-      parity ^= 1;
+    __syncwarp();  // the values are read, the next factors are written
+#pragma unroll
+    for (int t = 0; t < LT; ++t) mask[t] = next_mask[t];
+    if (more) {
+      copy(&k_map, sv);
+      copy_scales(n & 1);
+      ++issued;
+#pragma unroll
+      for (int t = 0; t < LT; ++t) next_mask[t] = cp_mask[t];
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    s = sv == 2 ? 0 : sv + 1;  // two boxes on
+    parity = sv == 2 ? parity_v ^ 1 : parity_v;
   }
   if (failed) {
     // A copy did not arrive: wait (bounded) for those in flight, give NaN.
-    for (int t = 0; t < S; ++t) {
+    for (int t = 0; t < 3; ++t) {
       (void)farq::mbar_wait_bounded(bars + 8 * s, parity, kAttnWaitNs);
-      if (++s == S) {
+      if (++s == 3) {
         s = 0;
         parity ^= 1;
       }
     }
-    l0 = l1 = __int_as_float(0x7fc00000);
+#pragma unroll
+    for (int x = 0; x < NB; ++x) l[x] = pair(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
   // Partial results into the warp's own ring, whose copies are all done.
-#pragma unroll
-  for (int x = 1; x <= 2; x <<= 1) {
-    l0 += __shfl_xor_sync(0xffffffffu, l0, x);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, x);
-  }
-  float4* const part = reinterpret_cast<float4*>(smem + L::ring + (size_t)warp * S * 2 * L::side);
   float* const ml = reinterpret_cast<float*>(smem + L::ml);
-  if (c == 0) {
-    float* const mine = ml + warp * 2 * kRows;
-    mine[g] = M0;
-    mine[g + 8] = M1;
-    mine[kRows + g] = l0;
-    mine[kRows + g + 8] = l1;
-  }
+  float4* const part = reinterpret_cast<float4*>(smem + L::ring + (size_t)warp * L::region);
 #pragma unroll
-  for (int x = 0; x < 2; ++x)
+  for (int x = 0; x < NB; ++x)
 #pragma unroll
-    for (int hh = 0; hh < NH; ++hh)
+    for (int e = 0; e < 2; ++e) {
+      float sum = e ? both(l[x]).y : both(l[x]).x;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {  // columns 2c and 2c + 1
-        constexpr int RUN = NT / NH;  // contiguous values of a column: 16, or 8 where D = 64
+      for (int y = 4; y <= 16; y <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, y);
+      const int row = 2 * c + e + 8 * x;
+      if (g == 0) {
+        ml[warp * 2 * R + row] = M[x][e];
+        ml[warp * 2 * R + R + row] = sum;
+      }
 #pragma unroll
-        for (int i = 0; i < RUN; i += 4) {
-          const int f4 = (hh * 128 + (2 * c + e) * RUN + i) / 4, t = hh * 16 + i;
-          part[part_index<D>(g + 8 * x, f4)] =
-              make_float4(o[t][2 * x + e], o[t + 1][2 * x + e], o[t + 2][2 * x + e], o[t + 3][2 * x + e]);
+      for (int hh = 0; hh < NH; ++hh) {
+        constexpr int RUN = NT / NH;  // tiles of a box: 8, or 4 where D = 64
+#pragma unroll
+        for (int i = 0; i < RUN; i += 2) {
+          const int f4 = (hh * 128 + g * 2 * RUN + 2 * i) / 4, t = hh * 8 + i;
+          part[part_index<D>(row, f4)] = make_float4(o[t][x][e], o[t][x][2 + e], o[t + 1][x][e], o[t + 1][x][2 + e]);
         }
       }
-  __syncthreads();
+    }
+  if (C > 1)
+    cluster_sync();
+  else
+    __syncthreads();
 
   // Join: maxima and sums of all warps first, then their outputs by weight.
+  // Every CTA of the cluster does so for its share of the output.
+  float* const all = reinterpret_cast<float*>(smem + L::all);
   float* const fin = reinterpret_cast<float*>(smem + L::fin);
-  if ((int)threadIdx.x < rows) {
-    const int row = threadIdx.x;
-    float m = -INFINITY, l = 0.f;
-    for (uint32_t n = 0; n < NW; ++n) m = fmaxf(m, ml[n * 2 * kRows + row]);
-    const float ms = m == -INFINITY ? 0.f : m;
-    for (uint32_t n = 0; n < NW; ++n) {
-      const float w = exp2_approx(ml[n * 2 * kRows + row] - ms);
-      l = fmaf(w, ml[n * 2 * kRows + kRows + row], l);
-      ml[n * 2 * kRows + row] = w;
-    }
-    fin[row] = l == 0.f ? 0.f : 1.0f / l;
-    if (p.lse)
-      p.lse[((int64_t)b * p.Q.d + qi) * p.H.d * p.G + head0 + row] =
-          l == 0.f ? -INFINITY : (m - kLift + log2f(l)) * 0.69314718055994531f;
+  for (uint32_t n = threadIdx.x; n < NW * 2 * R; n += kAttnThreads) {
+    const uint32_t src = n / (2 * R);
+    const uint32_t at = base + (uint32_t)L::ml + ((src % W) * 2 * R + n % (2 * R)) * 4;
+    all[n] = ld_cluster(mapa(at, src / W));
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < rows * (D / 4); i += W * 32) {
+  if ((int)threadIdx.x < rows) {
+    const int row = threadIdx.x;
+    float top = -INFINITY, sum = 0.f;
+    for (uint32_t n = 0; n < NW; ++n) top = fmaxf(top, all[n * 2 * R + row]);
+    const float from = top == -INFINITY ? 0.f : top;
+    for (uint32_t n = 0; n < NW; ++n) {
+      const float w = exp2_approx(all[n * 2 * R + row] - from);
+      sum = fmaf(w, all[n * 2 * R + R + row], sum);
+      all[n * 2 * R + row] = w;
+    }
+    fin[row] = sum == 0.f ? 0.f : 1.0f / sum;
+    if (p.lse && rank == 0)
+      p.lse[((int64_t)b * p.Q.d + qi) * p.H.d * p.G + head0 + row] =
+          sum == 0.f ? -INFINITY : (top - kLift + log2f(sum)) * 0.69314718055994531f;
+  }
+  __syncthreads();
+  for (int i = rank * kAttnThreads + threadIdx.x; i < rows * (D / 4); i += (int)C * kAttnThreads) {
     const int row = i / (D / 4), f4 = i % (D / 4);
     const uint32_t off = base + (uint32_t)L::ring + part_index<D>(row, f4) * 16;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (uint32_t n = 0; n < NW; ++n) {
-      const uint4 v = lds128(off + n * (uint32_t)(S * 2 * L::side));
-      const float w = ml[n * 2 * kRows + row];
-      acc.x = fmaf(w, __uint_as_float(v.x), acc.x);
-      acc.y = fmaf(w, __uint_as_float(v.y), acc.y);
-      acc.z = fmaf(w, __uint_as_float(v.z), acc.z);
-      acc.w = fmaf(w, __uint_as_float(v.w), acc.w);
+      const float4 v = ld_cluster4(mapa(off + (n % W) * (uint32_t)L::region, n / W));
+      const float w = all[n * 2 * R + row];
+      acc.x = fmaf(w, v.x, acc.x);
+      acc.y = fmaf(w, v.y, acc.y);
+      acc.z = fmaf(w, v.z, acc.z);
+      acc.w = fmaf(w, v.w, acc.w);
     }
     const float f = fin[row];
     uint2 v;
@@ -584,6 +757,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32)
     v.y = Half16<T>::pack(acc.z * f, acc.w * f);
     *reinterpret_cast<uint2*>(p.out.row(b, qi, head0 + row) + f4 * 8) = v;
   }
+  if (C > 1) cluster_sync();  // shared memory stays until every CTA has read it
 }
 
 }  // namespace kv

@@ -67,21 +67,26 @@ inline int check_cache(const dsa_kv_cache_t& c, bool written) {
   return DSA_KV_OK;
 }
 
-// Launch with programmatic stream serialisation: the kernel waits for the
-// previous one (griddepcontrol.wait) before its first global access.
+// Launch in clusters of `cluster` CTAs, with programmatic stream serialisation:
+// the kernel waits for the previous one (griddepcontrol.wait) before its first
+// global access.
 template <typename... A, typename... B>
-int launch(void (*fn)(A...), int64_t grid, int threads, size_t smem, void* stream, const B&... args) {
+int launch(void (*fn)(A...), int64_t grid, int threads, size_t smem, int cluster, void* stream, const B&... args) {
   if (grid > kMaxIndex) return DSA_KV_ERR_UNSUPPORTED;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, fn, args...) == cudaSuccess ? DSA_KV_OK : DSA_KV_ERR_CUDA;
 }
 
