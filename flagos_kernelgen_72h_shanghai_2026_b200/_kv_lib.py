@@ -158,22 +158,6 @@ def raise_status(op: str, status: int):
     raise ValueError(msg)
 
 
-def fast_launch(op: str, entry: str, tensors: tuple, *args) -> bool:
-    """Hand the call to the C++ launch path; False when it declines (it has then launched nothing)."""
-    if _fast is None:
-        return False
-    for t in tensors:
-        if type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
-            return False
-    try:
-        st = getattr(_fast, entry)(*tensors, *args)
-    except TypeError:  # a scalar pybind11 cannot convert: the checks of the Python path report it
-        return False
-    if st > 0:
-        raise_status(op, st)
-    return st == OK
-
-
 def launch(op: str, entry: str, args, device: torch.device) -> None:
     """Call a C entry point on the device's current stream; raise its error."""
     fn = getattr(load(), entry)

@@ -14,26 +14,12 @@ using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, voi
                               const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// The driver's tensor-map encoder, looked up once (the library does not link libcuda).
-EncodeFn encoder() {
-  static std::atomic<void*> fn{nullptr};
-  void* f = fn.load(std::memory_order_acquire);
-  if (!f) {
-    cudaDriverEntryPointQueryResult found;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) !=
-            cudaSuccess ||
-        found != cudaDriverEntryPointSuccess)
-      return nullptr;
-    fn.store(f, std::memory_order_release);
-  }
-  return reinterpret_cast<EncodeFn>(f);
-}
-
 // Map of the codes [P, H, block_size, D] as bytes: a box is `rows` tokens of
 // one head and page, 128 bytes wide (64 where D = 64), swizzled over its
 // width. Tokens behind the block read as zeros.
 bool make_map(CUtensorMap* map, const dsa_kv_cache_t& c, void* codes, const int64_t stride[3], int rows) {
-  EncodeFn encode = encoder();
+  static std::atomic<void*> entry{nullptr};
+  const EncodeFn encode = reinterpret_cast<EncodeFn>(driver_entry(&entry, "cuTensorMapEncodeTiled"));
   if (!encode) return false;
   const cuuint64_t dims[4] = {(cuuint64_t)c.D, (cuuint64_t)c.block_size, (cuuint64_t)c.H, (cuuint64_t)c.P};
   cuuint64_t strides[3] = {(cuuint64_t)stride[2], (cuuint64_t)stride[1], (cuuint64_t)stride[0]};
@@ -114,7 +100,7 @@ int attn(const dsa_kv_attn_args_t* a, void* stream) {
   const int box_rows = (int)(c.block_size < piece ? c.block_size : piece);
 
   int dev;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return DSA_KV_ERR_CUDA;
+  if (!bind_device(&dev) || dev < 0 || dev >= kMaxDevices) return DSA_KV_ERR_CUDA;
   int sms = g_sm_count[dev].load(std::memory_order_relaxed);
   if (sms <= 0) {
     if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return DSA_KV_ERR_CUDA;

@@ -14,6 +14,7 @@
 #include <torch/extension.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
 
 #include "dsa_kv.h"
 #include "dsa_topk.h"
@@ -278,7 +279,7 @@ bool selection(const at::Tensor& t, const dsa_kv_attn_args_t& a, const at::Devic
 // dsa_paged_attention (dsa_attention.py); returns dsa_kv_attn_launch's status or kNotHandled.
 int64_t kv_attn(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& k_scale, const at::Tensor& v_cache,
                 const at::Tensor& v_scale, const at::Tensor& blocks, const at::Tensor& pages, const at::Tensor& q_pos,
-                const at::Tensor& kv_lens, const at::Tensor& out, const c10::optional<at::Tensor>& lse,
+                const at::Tensor& kv_lens, const at::Tensor& out, const at::Tensor* lse,
                 double softmax_scale) {
   if (!q.defined() || !q.is_cuda() || q.dim() != 4 || !blocks.defined() || blocks.dim() != 4) return kNotHandled;
   const at::Device dev = q.device();
@@ -302,7 +303,7 @@ int64_t kv_attn(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor
   if (a.pos_dtype < 0 || kv_lens.scalar_type() != q_pos.scalar_type() || !is_2d(q_pos, a.B, a.Q) ||
       kv_lens.dim() != 1 || kv_lens.size(0) != a.B)
     return kNotHandled;
-  if (lse.has_value()) {
+  if (lse) {
     if (!same_cuda(*lse, dev) || lse->scalar_type() != at::kFloat || lse->dim() != 3 || lse->size(0) != a.B ||
         lse->size(1) != a.Q || lse->size(2) != Hq)
       return kNotHandled;
@@ -317,13 +318,73 @@ int64_t kv_attn(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor
   return dsa_kv_attn_launch(&a, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
 }
 
+// Entry points of the above without pybind11's argument conversion, which takes
+// about as long as the checks: positional arguments only, tensors (or
+// parameters) and nothing derived from them; anything else is not handled.
+bool tensors(PyObject* const* args, int n) {
+  for (int i = 0; i < n; ++i)
+    if (!THPVariable_CheckExact(args[i])) return false;
+  return true;
+}
+const at::Tensor& tensor(PyObject* o) { return THPVariable_Unpack(o); }
+bool number(PyObject* o, double* v) {
+  *v = PyFloat_AsDouble(o);
+  if (*v == -1.0 && PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  return true;
+}
+template <typename F>
+PyObject* answer(const F& f) {
+  int64_t st;
+  try {
+    st = f();
+  } catch (const std::exception& e) {  // of torch, for a device that is not there
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+  return PyLong_FromLongLong(st);
+}
+
+PyObject* py_kv_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  double eps;
+  if (n != 10 || !tensors(a, 8) || !number(a[8], &eps) || !PyBool_Check(a[9])) return PyLong_FromLong(kNotHandled);
+  return answer([&] {
+    return kv_rope(tensor(a[0]), tensor(a[1]), tensor(a[2]), tensor(a[3]), tensor(a[4]), tensor(a[5]), tensor(a[6]),
+                   tensor(a[7]), eps, a[9] == Py_True);
+  });
+}
+PyObject* py_kv_copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 9 || !tensors(a, 8) || !PyBool_Check(a[8])) return PyLong_FromLong(kNotHandled);
+  return answer([&] {
+    return kv_copy(tensor(a[0]), tensor(a[1]), tensor(a[2]), tensor(a[3]), tensor(a[4]), tensor(a[5]), tensor(a[6]),
+                   tensor(a[7]), a[8] == Py_True);
+  });
+}
+PyObject* py_kv_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  double scale;
+  if (n != 12 || !tensors(a, 10) || (a[10] != Py_None && !THPVariable_CheckExact(a[10])) || !number(a[11], &scale))
+    return PyLong_FromLong(kNotHandled);
+  return answer([&] {
+    return kv_attn(tensor(a[0]), tensor(a[1]), tensor(a[2]), tensor(a[3]), tensor(a[4]), tensor(a[5]), tensor(a[6]),
+                   tensor(a[7]), tensor(a[8]), tensor(a[9]), a[10] == Py_None ? nullptr : &tensor(a[10]), scale);
+  });
+}
+PyMethodDef kKvMethods[] = {
+    {"kv_rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&py_kv_rope)), METH_FASTCALL,
+     "checks + dsa_kv_rope_launch; status, or -1 when not handled"},
+    {"kv_copy", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&py_kv_copy)), METH_FASTCALL,
+     "checks + dsa_kv_write_launch / dsa_kv_read_launch; status, or -1 when not handled"},
+    {"kv_attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&py_kv_attn)), METH_FASTCALL,
+     "checks + dsa_kv_attn_launch; status, or -1 when not handled"},
+    {nullptr, nullptr, 0, nullptr}};
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "C++ launch path of the Python operators";
   m.def("task01", &task01, "checks + farq_launch; status, or -1 when not handled");
   m.def("task02", &task02, "checks + dsa_topk_launch; status, or -1 when not handled");
-  m.def("kv_rope", &kv_rope, "checks + dsa_kv_rope_launch; status, or -1 when not handled");
-  m.def("kv_copy", &kv_copy, "checks + dsa_kv_write_launch / dsa_kv_read_launch; status, or -1 when not handled");
-  m.def("kv_attn", &kv_attn, "checks + dsa_kv_attn_launch; status, or -1 when not handled");
+  if (PyModule_AddFunctions(m.ptr(), kKvMethods) != 0) throw py::error_already_set();
 }

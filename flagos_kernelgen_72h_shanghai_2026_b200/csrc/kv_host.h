@@ -1,8 +1,11 @@
 // kv_host.h — host-side checks and launch shared by the sources of libdsa_kv.so.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <atomic>
+#include <mutex>
 
 #include "dsa_kv.h"
 #include "kv_common.cuh"
@@ -67,27 +70,95 @@ inline int check_cache(const dsa_kv_cache_t& c, bool written) {
   return DSA_KV_OK;
 }
 
-// Launch in clusters of `cluster` CTAs, with programmatic stream serialisation:
-// the kernel waits for the previous one (griddepcontrol.wait) before its first
-// global access.
-template <typename... A, typename... B>
-int launch(void (*fn)(A...), int64_t grid, int threads, size_t smem, int cluster, void* stream, const B&... args) {
+// The current device, whose context is made the calling thread's: the driver's
+// own entry points do not do that for a thread's first call.
+inline bool bind_device(int* dev) {
+  thread_local int bound = -1;
+  if (cudaGetDevice(dev) != cudaSuccess) return false;
+  if (bound != *dev) {
+    if (cudaSetDevice(*dev) != cudaSuccess) return false;
+    bound = *dev;
+  }
+  return true;
+}
+
+// A driver entry point, looked up once (the library does not link libcuda).
+inline void* driver_entry(std::atomic<void*>* cached, const char* name) {
+  void* f = cached->load(std::memory_order_acquire);
+  if (f) return f;
+  cudaDriverEntryPointQueryResult found;
+  if (cudaGetDriverEntryPointByVersion(name, &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+      found != cudaDriverEntryPointSuccess)
+    return nullptr;
+  cached->store(f, std::memory_order_release);
+  return f;
+}
+
+// The driver's handle of a kernel on a device: a table that is only ever added
+// to. Launching by it skips the runtime's own look-up of the kernel on every
+// call.
+inline CUfunction kernel_handle(const void* fn, int dev) {
+  constexpr int kSlots = 1024;
+  struct Slot {
+    std::atomic<const void*> fn;
+    std::atomic<int> dev;
+    std::atomic<CUfunction> handle;
+  };
+  static Slot table[kSlots];
+  static std::mutex lock;
+  const size_t at = ((reinterpret_cast<uintptr_t>(fn) >> 4) + (size_t)dev * 131) % kSlots;
+  for (size_t i = at, n = 0; n < kSlots; ++n, i = (i + 1) % kSlots) {
+    const void* have = table[i].fn.load(std::memory_order_acquire);
+    if (!have) break;
+    if (have == fn && table[i].dev.load(std::memory_order_relaxed) == dev)
+      return table[i].handle.load(std::memory_order_relaxed);
+  }
+  cudaFunction_t f;
+  if (cudaGetFuncBySymbol(&f, fn) != cudaSuccess) return nullptr;
+  std::lock_guard<std::mutex> hold(lock);
+  for (size_t i = at, n = 0; n < kSlots; ++n, i = (i + 1) % kSlots) {
+    const void* have = table[i].fn.load(std::memory_order_relaxed);
+    if (have == fn && table[i].dev.load(std::memory_order_relaxed) == dev) break;
+    if (have) continue;
+    table[i].dev.store(dev, std::memory_order_relaxed);
+    table[i].handle.store(f, std::memory_order_relaxed);
+    table[i].fn.store(fn, std::memory_order_release);
+    break;
+  }
+  return f;
+}
+
+// Launch on the current device, in clusters of `cluster` CTAs, with
+// programmatic stream serialisation: the kernel waits for the previous one
+// (griddepcontrol.wait) before its first global access.
+template <typename... A>
+int launch(void (*fn)(A...), int64_t grid, int threads, size_t smem, int cluster, void* stream, const A&... args) {
   if (grid > kMaxIndex) return DSA_KV_ERR_UNSUPPORTED;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)cluster;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
+  static std::atomic<void*> entry{nullptr};
+  using LaunchFn = CUresult (*)(const CUlaunchConfig*, CUfunction, void**, void**);
+  const LaunchFn launch_ex = reinterpret_cast<LaunchFn>(driver_entry(&entry, "cuLaunchKernelEx"));
+  int dev;
+  if (!launch_ex || !bind_device(&dev)) return DSA_KV_ERR_CUDA;
+  const CUfunction f = kernel_handle(reinterpret_cast<const void*>(fn), dev);
+  if (!f) return DSA_KV_ERR_CUDA;
+  CUlaunchAttribute attr[2] = {};
+  attr[0].id = CU_LAUNCH_ATTRIBUTE_PROGRAMMATIC_STREAM_SERIALIZATION;
+  attr[0].value.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = CU_LAUNCH_ATTRIBUTE_CLUSTER_DIMENSION;
+  attr[1].value.clusterDim.x = (unsigned)cluster;
+  attr[1].value.clusterDim.y = 1;
+  attr[1].value.clusterDim.z = 1;
+  CUlaunchConfig cfg = {};
+  cfg.gridDimX = (unsigned)grid;
+  cfg.gridDimY = cfg.gridDimZ = 1;
+  cfg.blockDimX = (unsigned)threads;
+  cfg.blockDimY = cfg.blockDimZ = 1;
+  cfg.sharedMemBytes = (unsigned)smem;
+  cfg.hStream = static_cast<CUstream>(stream);
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, fn, args...) == cudaSuccess ? DSA_KV_OK : DSA_KV_ERR_CUDA;
+  void* params[] = {const_cast<void*>(static_cast<const void*>(&args))...};
+  return launch_ex(&cfg, f, params, nullptr) == CUDA_SUCCESS ? DSA_KV_OK : DSA_KV_ERR_CUDA;
 }
 
 }  // namespace kv

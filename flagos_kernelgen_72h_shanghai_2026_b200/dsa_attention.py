@@ -49,9 +49,13 @@ def dsa_paged_attention(q: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.T
     padded one (negative position), has out = 0 and lse = -inf.
 
     D is 64, 128 or 256; block_size is 8 to 65536."""
-    if L.fast_launch(_OP, "kv_attn", (q, k_cache, k_scale, v_cache, v_scale, blocks, pages, q_pos,
-                                      kv_lens, out), lse, softmax_scale):
-        return out, lse
+    if L._fast is not None:
+        st = L._fast.kv_attn(q, k_cache, k_scale, v_cache, v_scale, blocks, pages, q_pos, kv_lens, out, lse,
+                             softmax_scale)
+        if st == 0:
+            return out, lse
+        if st > 0:
+            L.raise_status(_OP, st)
     dev = L.check_tensor("q", q, None)
     a = L.AttnArgs()
     a.struct_size = ctypes.sizeof(a)

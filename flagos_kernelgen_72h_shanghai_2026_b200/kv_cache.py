@@ -68,9 +68,12 @@ def paged_kv_quant_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor
     NB * block_size, or if its page id is not in [0, P). The tokens of a call
     have cells of their own: of two for the same cell, which remains is not
     specified, and it may be one's codes with the other's scale."""
-    if L.fast_launch("paged_kv_quant_write", "kv_copy",
-                     (k, v, k_cache, k_scale, v_cache, v_scale, page_table, q_pos), True):
-        return k_cache, k_scale, v_cache, v_scale
+    if L._fast is not None:
+        st = L._fast.kv_copy(k, v, k_cache, k_scale, v_cache, v_scale, page_table, q_pos, True)
+        if st == 0:
+            return k_cache, k_scale, v_cache, v_scale
+        if st > 0:
+            L.raise_status("paged_kv_quant_write", st)
     a, dev = _args(k, v, ("k", "v"), k_cache, k_scale, v_cache, v_scale, page_table, q_pos,
                    "q_pos", 2)
     L.launch("paged_kv_quant_write", "dsa_kv_write_launch", a, dev)
@@ -84,9 +87,12 @@ def paged_kv_dequant_read(k_cache: torch.Tensor, k_scale: torch.Tensor, v_cache:
     sequence into k_out, v_out [B, S, H, D] (bf16 or fp16, rows on 16 bytes);
     returns both. Rows behind a sequence's end are left as they are; a token
     whose page id is not in [0, P) reads as zeros."""
-    if L.fast_launch("paged_kv_dequant_read", "kv_copy",
-                     (k_out, v_out, k_cache, k_scale, v_cache, v_scale, page_table, kv_lens), False):
-        return k_out, v_out
+    if L._fast is not None:
+        st = L._fast.kv_copy(k_out, v_out, k_cache, k_scale, v_cache, v_scale, page_table, kv_lens, False)
+        if st == 0:
+            return k_out, v_out
+        if st > 0:
+            L.raise_status("paged_kv_dequant_read", st)
     a, dev = _args(k_out, v_out, ("k_out", "v_out"), k_cache, k_scale, v_cache, v_scale,
                    page_table, kv_lens, "kv_lens", 1)
     L.launch("paged_kv_dequant_read", "dsa_kv_read_launch", a, dev)

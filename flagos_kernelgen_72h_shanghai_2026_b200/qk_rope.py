@@ -36,9 +36,12 @@ def qk_rmsnorm_rope(q: torch.Tensor, k: torch.Tensor, q_gamma: torch.Tensor, k_g
     values, in fp32; outputs are rounded once.
 
     D % 8 == 0, D <= 256; rot % 16 == 0 (interleaved: rot % 8 == 0)."""
-    if L.fast_launch(_OP, "kv_rope", (q, k, q_gamma, k_gamma, cos_sin, positions, q_out, k_out),
-                     eps, bool(interleaved)):
-        return q_out, k_out
+    if L._fast is not None:
+        st = L._fast.kv_rope(q, k, q_gamma, k_gamma, cos_sin, positions, q_out, k_out, eps, interleaved)
+        if st == 0:
+            return q_out, k_out
+        if st > 0:
+            L.raise_status(_OP, st)
     dev = L.check_tensor("q", q, None)
     dt = L.dtype_code("q", q, L.HALF_DTYPES)
     if q.dim() != 4:

@@ -13,7 +13,9 @@ them, n tokens, D the head size):
   sums     over n tokens: n/16 steps of 17 terms as above.
   q        bf16 and fp16 values are exact down to 2^-28 of the tile's largest.
 """
+import ctypes
 import math
+import threading
 
 import pytest
 import torch
@@ -416,6 +418,58 @@ def test_calls_on_two_streams(dev):
     torch.cuda.synchronize(dev)
     for (o, l), (wo, wl) in zip(outs, want):
         assert torch.equal(o, wo) and torch.equal(l, wl)
+
+
+def test_calls_from_other_threads(dev):
+    """Threads that have made no CUDA call of their own, several at once, each on its own stream."""
+    x = inputs(43, B=2, Q=4)
+    want = run(dev, x[4], x[3], *x[5:], 0.1)
+    args = [t.to(dev) for t in (x[4], *x[3], *x[5:])]
+    outs = [(torch.zeros_like(args[0]), torch.zeros(x[4].shape[:3], device=dev)) for _ in range(4)]
+    streams = [torch.cuda.Stream(dev) for _ in outs]
+    torch.cuda.synchronize(dev)
+    errors = []
+
+    def work(o, stream):
+        try:
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    dsa_paged_attention(*args, *o, 0.1)
+        except Exception as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(outs, streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize(dev)
+    assert not errors, errors
+    for o, l in outs:
+        assert torch.equal(o, want[0]) and torch.equal(l, want[1])
+
+
+def test_a_first_call_from_a_thread_without_a_context(dev):
+    """The C entry point called from a thread that has made no CUDA call at all."""
+    from flagos_kernelgen_72h_shanghai_2026_b200 import _kv_lib as L
+    q = torch.randn(1, 2, 4, 64, device=dev).to(BF16)
+    gamma, cs = torch.ones(64, device=dev), angles(8, 64).to(dev)
+    pos = torch.zeros(1, 2, dtype=torch.int32, device=dev)
+    want, out = torch.empty_like(q), torch.zeros_like(q)
+    k = torch.empty(1, 2, 0, 64, dtype=BF16, device=dev)
+    qk_rmsnorm_rope(q, k, gamma, gamma, cs, pos, want, k, 1e-6)
+    torch.cuda.synchronize(dev)
+    a = L.RopeArgs(struct_size=ctypes.sizeof(L.RopeArgs), dtype=L.DTYPE_BF16, gamma_dtype=L.DTYPE_FP32,
+                   pos_dtype=L.DTYPE_INT32, eps=1e-6, B=1, Q=2, Hq=4, Hk=0, D=64, rot=64, max_pos=8)
+    a.q, a.q_out = L.Dense(q.data_ptr(), *q.stride()[:3]), L.Dense(out.data_ptr(), *out.stride()[:3])
+    a.q_gamma = a.k_gamma = gamma.data_ptr()
+    a.cos_sin, a.positions = cs.data_ptr(), pos.data_ptr()
+    lib, got = L.load(), []
+    t = threading.Thread(target=lambda: got.append(lib.dsa_kv_rope_launch(ctypes.byref(a), None)))
+    t.start()
+    t.join()
+    torch.cuda.synchronize(dev)
+    assert got == [L.OK] and torch.equal(out, want)
 
 
 def test_a_long_row(dev):
