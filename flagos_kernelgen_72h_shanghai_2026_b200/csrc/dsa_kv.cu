@@ -23,14 +23,6 @@ CacheSide side(void* codes, float* scale, const int64_t s[3], const int64_t ss[3
 
 int lanes_of(int64_t D) { return D <= 64 ? 8 : D <= 128 ? 16 : 32; }
 
-// Heads per step and steps per task of the rotation, measured at 8192 tokens x
-// (32 + 8) heads x 128 (bf16; us with 1 / 2 / 4 tasks' worth of steps): 1 head
-// per lane group at a time 73.8; 2: 53.0 / 41.6 / -; 4: 44.3 / 38.3 / 39.6.
-// More steps spread the token's factors over more heads, until too few warps
-// are left; one token's 40 heads take 4.4 us with any of them.
-constexpr int kRopeUnroll = 4;
-constexpr int kRopeSteps = 2;
-
 using RopeFn = void (*)(const RopeParams);
 template <typename T, bool I>
 RopeFn rope_fn(int lanes) {
@@ -80,8 +72,8 @@ int rope(const dsa_kv_rope_args_t* a, void* stream) {
       !aligned(a->positions, ib))
     return DSA_KV_ERR_ALIGNMENT;
 
-  const int lanes = lanes_of(a->D), strip = 32 / lanes * kRopeUnroll * kRopeSteps;
-  const int64_t sq = ceil_div(a->Hq, strip), strips = sq + ceil_div(a->Hk, strip);
+  const int lanes = lanes_of(a->D), heads = 32 / lanes * kRopeUnroll;  // of a step
+  const int64_t steps_q = ceil_div(a->Hq, heads), per_token = steps_q + ceil_div(a->Hk, heads);
   RopeParams p;
   p.q = dense(a->q);
   p.k = dense(a->k);
@@ -92,11 +84,11 @@ int rope(const dsa_kv_rope_args_t* a, void* stream) {
   p.cos_sin = a->cos_sin;
   p.positions = a->positions;
   p.max_pos = a->max_pos;
-  p.tasks = (uint32_t)(a->B * a->Q * strips);
-  p.strips.init((uint32_t)strips);
+  p.tokens = (uint32_t)(a->B * a->Q);
+  p.steps = (uint32_t)(a->B * a->Q * per_token);
+  p.per_token.init((uint32_t)per_token);
   p.Q.init((uint32_t)a->Q);
-  p.strips_q = (uint32_t)sq;
-  p.strip = (uint32_t)strip;
+  p.steps_q = (uint32_t)steps_q;
   p.Hq = (uint32_t)a->Hq;
   p.Hk = (uint32_t)a->Hk;
   p.D = (int32_t)a->D;
@@ -108,7 +100,11 @@ int rope(const dsa_kv_rope_args_t* a, void* stream) {
   const RopeFn fn = a->dtype == DSA_KV_BF16
                         ? (a->interleaved ? rope_fn<__nv_bfloat16, true>(lanes) : rope_fn<__nv_bfloat16, false>(lanes))
                         : (a->interleaved ? rope_fn<__half, true>(lanes) : rope_fn<__half, false>(lanes));
-  return launch(fn, ceil_div(p.tasks, kCtaWarps), kCtaThreads, 0, 1, stream, p);
+  // A warp for every step, as far as they are all resident at once.
+  int dev, sms;
+  if (!bind_device(&dev) || !sm_count(dev, &sms)) return DSA_KV_ERR_CUDA;
+  const int64_t most = (int64_t)sms * kRopeCtas, grid = ceil_div(p.steps, kCtaWarps);
+  return launch(fn, grid < most ? grid : most, kCtaThreads, 0, 1, stream, p);
 }
 
 int copy(const dsa_kv_copy_args_t* a, void* stream, bool write) {

@@ -7,7 +7,6 @@
 
 namespace kv {
 
-constexpr int kMaxDevices = 64;
 constexpr int64_t kMaxBlockSize = 65536;
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -55,7 +54,6 @@ Variant variant_of(int64_t D, int nb) {
   return nb == 1 ? variant<T, E, 256, 1, 32, 2>() : variant<T, E, 256, 2, 32, 1>();
 }
 
-std::atomic<int> g_sm_count[kMaxDevices];
 // Shared memory granted to each variant, per device.
 std::atomic<bool> g_granted[kMaxDevices][24];
 
@@ -99,13 +97,8 @@ int attn(const dsa_kv_attn_args_t* a, void* stream) {
   if (a->K > (1 << 30) || items > (1 << 30)) return DSA_KV_ERR_UNSUPPORTED;
   const int box_rows = (int)(c.block_size < piece ? c.block_size : piece);
 
-  int dev;
-  if (!bind_device(&dev) || dev < 0 || dev >= kMaxDevices) return DSA_KV_ERR_CUDA;
-  int sms = g_sm_count[dev].load(std::memory_order_relaxed);
-  if (sms <= 0) {
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return DSA_KV_ERR_CUDA;
-    g_sm_count[dev].store(sms, std::memory_order_relaxed);
-  }
+  int dev, sms;
+  if (!bind_device(&dev) || !sm_count(dev, &sms)) return DSA_KV_ERR_CUDA;
   std::atomic<bool>& granted = g_granted[dev][(c.D / 128) * 8 + (nb - 1) * 4 + (e ? 2 : 0) + (bf ? 1 : 0)];
   if (!granted.load(std::memory_order_relaxed)) {
     if (cudaFuncSetAttribute(reinterpret_cast<const void*>(v.fn), cudaFuncAttributeMaxDynamicSharedMemorySize,

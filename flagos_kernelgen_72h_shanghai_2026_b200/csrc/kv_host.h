@@ -82,6 +82,17 @@ inline bool bind_device(int* dev) {
   return true;
 }
 
+constexpr int kMaxDevices = 64;
+inline bool sm_count(int dev, int* sms) {
+  static std::atomic<int> known[kMaxDevices];
+  if (dev < 0 || dev >= kMaxDevices) return false;
+  *sms = known[dev].load(std::memory_order_relaxed);
+  if (*sms > 0) return true;
+  if (cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return false;
+  known[dev].store(*sms, std::memory_order_relaxed);
+  return true;
+}
+
 // A driver entry point, looked up once (the library does not link libcuda).
 inline void* driver_entry(std::atomic<void*>* cached, const char* name) {
   void* f = cached->load(std::memory_order_acquire);
