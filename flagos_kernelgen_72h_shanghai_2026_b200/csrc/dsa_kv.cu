@@ -103,8 +103,8 @@ int rope(const dsa_kv_rope_args_t* a, void* stream) {
   // A warp for every step, as far as they are all resident at once.
   int dev, sms;
   if (!bind_device(&dev) || !sm_count(dev, &sms)) return DSA_KV_ERR_CUDA;
-  const int64_t most = (int64_t)sms * kRopeCtas, grid = ceil_div(p.steps, kCtaWarps);
-  return launch(fn, grid < most ? grid : most, kCtaThreads, 0, 1, stream, p);
+  const int64_t most = (int64_t)sms * kRopeCtas, grid = ceil_div(p.steps, kRopeWarps);
+  return launch(fn, grid < most ? grid : most, kRopeThreads, 0, 1, stream, p);
 }
 
 int copy(const dsa_kv_copy_args_t* a, void* stream, bool write) {
@@ -161,7 +161,7 @@ int copy(const dsa_kv_copy_args_t* a, void* stream, bool write) {
   const CopyFn fn = a->dtype == DSA_KV_BF16
                         ? (e ? copy_fn<__nv_bfloat16, true>(lanes, write, u) : copy_fn<__nv_bfloat16, false>(lanes, write, u))
                         : (e ? copy_fn<__half, true>(lanes, write, u) : copy_fn<__half, false>(lanes, write, u));
-  return launch(fn, ceil_div(p.tasks, kCtaWarps), kCtaThreads, 0, 1, stream, p);
+  return launch(fn, ceil_div(p.tasks, kCopyThreads / 32), kCopyThreads, 0, 1, stream, p);
 }
 
 }  // namespace kv

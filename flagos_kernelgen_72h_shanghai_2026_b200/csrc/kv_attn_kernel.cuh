@@ -99,8 +99,8 @@ struct AttnSmem {
   static constexpr bool q_in_smem = D == 256 && NB == 2;             // where the output fills the registers
   static constexpr size_t qf = fin + R * 4;
   static constexpr size_t all = qf + (q_in_smem ? (size_t)(D / 16) * NB * 32 * 8 : 0);
-  // [C * W][2][R] of the cluster, then weights
-  static constexpr size_t total(int cluster) { return all + (size_t)cluster * W * 2 * R * 4; }
+  // [C * W][R] weights of the cluster's warps
+  static constexpr size_t total(int cluster) { return all + (size_t)cluster * W * R * 4; }
 };
 
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int tok, int head, int page,
@@ -712,50 +712,82 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
   else
     __syncthreads();
 
-  // Join: maxima and sums of all warps first, then their outputs by weight.
-  // Every CTA of the cluster does so for its share of the output.
+  // Join. Every CTA of the cluster works out the weights of all NW warps, a
+  // group of lanes per head, and then its share of the output, as many lanes to
+  // four values as there are to spare. (A thread per head and per four values
+  // took 2 us longer with 32 warps: each walked through all of them.)
   float* const all = reinterpret_cast<float*>(smem + L::all);
   float* const fin = reinterpret_cast<float*>(smem + L::fin);
-  for (uint32_t n = threadIdx.x; n < NW * 2 * R; n += kAttnThreads) {
-    const uint32_t src = n / (2 * R);
-    const uint32_t at = base + (uint32_t)L::ml + ((src % W) * 2 * R + n % (2 * R)) * 4;
-    all[n] = ld_cluster(mapa(at, src / W));
-  }
-  __syncthreads();
-  if ((int)threadIdx.x < rows) {
-    const int row = threadIdx.x;
-    float top = -INFINITY, sum = 0.f;
-    for (uint32_t n = 0; n < NW; ++n) top = fmaxf(top, all[n * 2 * R + row]);
-    const float from = top == -INFINITY ? 0.f : top;
-    for (uint32_t n = 0; n < NW; ++n) {
-      const float w = exp2_approx(all[n * 2 * R + row] - from);
-      sum = fmaf(w, all[n * 2 * R + R + row], sum);
-      all[n * 2 * R + row] = w;
+  {
+    constexpr int LPR = kAttnThreads / R;  // lanes of a head: 16 or 8
+    constexpr int MOST = kMaxCluster * W / LPR;
+    const int row = threadIdx.x / LPR;
+    const uint32_t sub = threadIdx.x % LPR;
+    float top[MOST], sum[MOST], m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+      const uint32_t n = sub + i * LPR;
+      top[i] = -INFINITY;
+      sum[i] = 0.f;
+      if (n < NW) {
+        const uint32_t at = mapa(base + (uint32_t)L::ml + ((n % W) * 2 * R + row) * 4, n / W);
+        top[i] = ld_cluster(at);
+        sum[i] = ld_cluster(at + R * 4);
+      }
+      m = fmaxf(m, top[i]);
     }
-    fin[row] = sum == 0.f ? 0.f : 1.0f / sum;
-    if (p.lse && rank == 0)
-      p.lse[((int64_t)b * p.Q.d + qi) * p.H.d * p.G + head0 + row] =
-          sum == 0.f ? -INFINITY : (top - kLift + log2f(sum)) * 0.69314718055994531f;
+#pragma unroll
+    for (int y = 1; y < LPR; y <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, y));
+    const float from_all = m == -INFINITY ? 0.f : m;
+    float total = 0.f;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+      const uint32_t n = sub + i * LPR;
+      const float w = exp2_approx(top[i] - from_all);
+      total = fmaf(w, sum[i], total);
+      if (n < NW) all[n * R + row] = w;
+    }
+#pragma unroll
+    for (int y = 1; y < LPR; y <<= 1) total += __shfl_xor_sync(0xffffffffu, total, y);
+    if (sub == 0) {
+      fin[row] = total == 0.f ? 0.f : 1.0f / total;
+      if (p.lse && rank == 0 && row < rows)
+        p.lse[((int64_t)b * p.Q.d + qi) * p.H.d * p.G + head0 + row] =
+            total == 0.f ? -INFINITY : (m - kLift + log2f(total)) * 0.69314718055994531f;
+    }
   }
   __syncthreads();
-  for (int i = rank * kAttnThreads + threadIdx.x; i < rows * (D / 4); i += (int)C * kAttnThreads) {
-    const int row = i / (D / 4), f4 = i % (D / 4);
+  const int units = rows * (D / 4), share = (units + (int)C - 1) / (int)C;
+  int log_lanes = 0;
+  while (log_lanes < 4 && (2u << log_lanes) <= NW && (share << (log_lanes + 1)) <= kAttnThreads) ++log_lanes;
+  for (int i0 = 0; i0 < share; i0 += kAttnThreads >> log_lanes) {
+    const int i = rank * share + i0 + (threadIdx.x >> log_lanes);
+    const bool mine = i0 + (int)(threadIdx.x >> log_lanes) < share && i < units;
+    const int row = mine ? i / (D / 4) : 0, f4 = mine ? i % (D / 4) : 0;
     const uint32_t off = base + (uint32_t)L::ring + part_index<D>(row, f4) * 16;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (uint32_t n = 0; n < NW; ++n) {
+    for (uint32_t n = threadIdx.x & ((1u << log_lanes) - 1); n < NW; n += 1u << log_lanes) {
       const float4 v = ld_cluster4(mapa(off + (n % W) * (uint32_t)L::region, n / W));
-      const float w = all[n * 2 * R + row];
+      const float w = all[n * R + row];
       acc.x = fmaf(w, v.x, acc.x);
       acc.y = fmaf(w, v.y, acc.y);
       acc.z = fmaf(w, v.z, acc.z);
       acc.w = fmaf(w, v.w, acc.w);
     }
-    const float f = fin[row];
-    uint2 v;
-    v.x = Half16<T>::pack(acc.x * f, acc.y * f);
-    v.y = Half16<T>::pack(acc.z * f, acc.w * f);
-    *reinterpret_cast<uint2*>(p.out.row(b, qi, head0 + row) + f4 * 8) = v;
+    for (int y = 1; y < 1 << log_lanes; y <<= 1) {
+      acc.x += __shfl_xor_sync(0xffffffffu, acc.x, y);
+      acc.y += __shfl_xor_sync(0xffffffffu, acc.y, y);
+      acc.z += __shfl_xor_sync(0xffffffffu, acc.z, y);
+      acc.w += __shfl_xor_sync(0xffffffffu, acc.w, y);
+    }
+    if (mine && (threadIdx.x & ((1u << log_lanes) - 1)) == 0) {
+      const float f = fin[row];
+      uint2 v;
+      v.x = Half16<T>::pack(acc.x * f, acc.y * f);
+      v.y = Half16<T>::pack(acc.z * f, acc.w * f);
+      *reinterpret_cast<uint2*>(p.out.row(b, qi, head0 + row) + f4 * 8) = v;
+    }
   }
   if (C > 1) cluster_sync();  // shared memory stays until every CTA has read it
 }

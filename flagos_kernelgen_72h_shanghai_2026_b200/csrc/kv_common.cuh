@@ -11,8 +11,6 @@
 
 namespace kv {
 
-constexpr int kCtaThreads = 256;  // of the three copying kernels
-constexpr int kCtaWarps = kCtaThreads / 32;
 constexpr float kMinScale = 1.0e-12f;
 
 // Division of n < 2^31 by d >= 1 with a precomputed multiplier (the round-up

@@ -25,6 +25,7 @@
 namespace kv {
 
 constexpr int kRopeUnroll = 4;  // heads that a group of lanes holds at a time
+constexpr int kRopeThreads = 256, kRopeWarps = kRopeThreads / 32;
 constexpr int kRopeCtas = 2;    // CTAs per SM
 
 struct RopeParams {
@@ -63,11 +64,11 @@ __device__ __forceinline__ void load_gamma8(const void* g, int i, int dtype, flo
 // next step's values (and, where they change, its angles) on the way while it
 // works on this one.
 template <typename T, int LPH, int U, bool INTERLEAVED>
-__global__ void __launch_bounds__(kCtaThreads, kRopeCtas) rope_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(kRopeThreads, kRopeCtas) rope_kernel(const RopeParams p) {
   constexpr int HPW = 32 / LPH;
   constexpr int NA = INTERLEAVED ? 4 : 8;  // angles of a lane's values
   pdl_wait();
-  const uint32_t warps = gridDim.x * kCtaWarps, warp = blockIdx.x * kCtaWarps + (threadIdx.x >> 5);
+  const uint32_t warps = gridDim.x * kRopeWarps, warp = blockIdx.x * kRopeWarps + (threadIdx.x >> 5);
   uint32_t step = (uint32_t)((uint64_t)p.steps * warp / warps);
   const uint32_t last = (uint32_t)((uint64_t)p.steps * (warp + 1) / warps);
   if (step == last) return;
