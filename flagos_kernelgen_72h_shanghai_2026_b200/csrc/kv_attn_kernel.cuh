@@ -296,6 +296,22 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     }
     const int first = __ffs(active) - 1;
     active &= active - 1;
+    if (lp == 0) {
+      cp_page = __shfl_sync(0xffffffffu, pc_page, first);
+      cp_off = __shfl_sync(0xffffffffu, pc_off, first);
+      const int n = __shfl_sync(0xffffffffu, pc_n, first);
+      cp_bytes = NH * p.box_bytes;
+      copies = lane == 0;
+      cp_ks[0] = k_scale + (uint64_t)(uint32_t)cp_page * p.ksp + (uint64_t)(uint32_t)(cp_off + lane) * p.kst;
+      cp_vs[0] = v_scale + (uint64_t)(uint32_t)cp_page * p.vsp + (uint64_t)(uint32_t)(cp_off + lane) * p.vst;
+      cp_mask[0] = n >= 32 ? 0xffffffffu : (1u << n) - 1;
+      if (LT == 2) {
+        cp_ks[LT - 1] = cp_ks[0] + (uint64_t)p.kst * 32;
+        cp_vs[LT - 1] = cp_vs[0] + (uint64_t)p.vst * 32;
+        cp_mask[LT - 1] = n >= 64 ? 0xffffffffu : n > 32 ? (1u << (n - 32)) - 1 : 0;
+      }
+      return;
+    }
     const uint32_t here = (pieces >> first) & ((1u << per) - 1);
     cp_bytes = __popc(here) * NH * p.box_bytes;
     copies = lane < per && ((here >> lane) & 1);
@@ -311,10 +327,12 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     cp_page = __shfl_sync(0xffffffffu, pc_page, first + lane);
     cp_off = __shfl_sync(0xffffffffu, pc_off, first + lane);
   };
+  uint32_t started = 0;  // copies so far: the i-th fills box i % 3
   auto copy = [&](const CUtensorMap* map, int s) {
     const uint32_t bar = bars + 8 * s;
+    ++started;
     if (lane == 0) farq::mbar_arrive_expect_tx(bar, cp_bytes);
-    __syncwarp();
+    if (lp != 0) __syncwarp();  // other lanes copy too
     if (copies) {
       const uint32_t dst = farq::smem_u32(ring) + s * (uint32_t)L::box + lane * pitch * ROWB;
 #pragma unroll
@@ -479,11 +497,8 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     const uint32_t parity_v = s == 2 ? parity ^ 1 : parity;
     uint8_t* const kbox = ring + s * L::box;
     uint8_t* const vbox = ring + sv * L::box;
-    if (!farq::mbar_wait_bounded(bars + 8 * s, parity, kAttnWaitNs)) failed = true;
-    if (__any_sync(0xffffffffu, failed)) {
-      failed = true;
-      break;
-    }
+    // a wait that runs out ends the loop before the next copy
+    failed = !farq::mbar_wait_bounded(bars + 8 * s, parity, kAttnWaitNs);
     clear(kbox, mask);
 
     // scores: tile t has tokens 16t + g and 16t + g + 8 as this lane's rows
@@ -532,6 +547,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
         }
       }
     __syncwarp();  // the keys are read
+    if (__any_sync(0xffffffffu, failed)) break;
     if (n + 1 < issued) copy(&v_map, s);
     if (more) prepare();
 
@@ -611,11 +627,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     factors((n & 1) ^ 1);
 
-    if (!farq::mbar_wait_bounded(bars + 8 * sv, parity_v, kAttnWaitNs)) failed = true;
-    if (__any_sync(0xffffffffu, failed)) {
-      failed = true;
-      break;
-    }
+    failed |= !farq::mbar_wait_bounded(bars + 8 * sv, parity_v, kAttnWaitNs);
     clear(vbox, mask);
     // values times weights; rows g and g + 8 of output tile y are values
     // 16g + 2y and 16g + 2y + 1 of their box (8g + .. where D = 64)
@@ -653,6 +665,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
       }
     }
     __syncwarp();  // the values are read, the next factors are written
+    if (__any_sync(0xffffffffu, failed)) break;
 #pragma unroll
     for (int t = 0; t < LT; ++t) mask[t] = next_mask[t];
     if (more) {
@@ -666,15 +679,10 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     s = sv == 2 ? 0 : sv + 1;  // two boxes on
     parity = sv == 2 ? parity_v ^ 1 : parity_v;
   }
-  if (failed) {
+  if (__any_sync(0xffffffffu, failed)) {
     // A copy did not arrive: wait (bounded) for those in flight, give NaN.
-    for (int t = 0; t < 3; ++t) {
-      (void)farq::mbar_wait_bounded(bars + 8 * s, parity, kAttnWaitNs);
-      if (++s == 3) {
-        s = 0;
-        parity ^= 1;
-      }
-    }
+    for (uint32_t i = started < 3 ? 0 : started - 3; i < started; ++i)
+      (void)farq::mbar_wait_bounded(bars + 8 * (i % 3), (i / 3) & 1, kAttnWaitNs);
 #pragma unroll
     for (int x = 0; x < NB; ++x) l[x] = pair(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
   }
