@@ -8,6 +8,7 @@
 namespace kv {
 
 constexpr int64_t kMaxBlockSize = 65536;
+constexpr size_t kSmemPerSm = 228 * 1024, kSmemReserved = 1024;  // of an SM; of it for each CTA, by the system
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                               const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -42,16 +43,18 @@ Variant variant() {
   using L = AttnSmem<D, NB, TOK>;
   return Variant{attn_kernel<T, D, E, NB, TOK, CTAS>, L::total(1), L::total(2) - L::total(1), TOK, CTAS};
 }
-// Tokens of a chunk and CTAs per SM. A ring of three boxes of 64 tokens leaves
-// room for two CTAs at D = 128. Measured there with 16 heads (us, 1024 rows x
-// 2048 tokens): 64 tokens and 2 CTAs 95.7, 32 tokens and 3 CTAs 108.5, 32
-// tokens and 2 CTAs 118: what a chunk costs besides its products weighs more
-// than the warps that hide it.
+// Tokens of a chunk, and CTAs per SM that registers are laid out for. Measured
+// (us): chunks of 64 tokens against 32 with 16 heads at D = 128, 1024 rows x
+// 2048 tokens: 95.7 against 108.5 (three CTAs of 32) and 118 (two): what a chunk
+// costs besides its products weighs more than the warps that hide it. Three
+// CTAs against two there: 100.4 against 94.9; with 8 heads, 2048 rows: 116
+// against 134; at D = 64, 2048 rows: 74 (four) against 81 (three) with 8 heads,
+// 104 (three) against 122 (two) with 16.
 template <typename T, bool E>
 Variant variant_of(int64_t D, int nb) {
-  if (D == 64) return nb == 1 ? variant<T, E, 64, 1, 64, 3>() : variant<T, E, 64, 2, 64, 2>();
-  if (D == 128) return nb == 1 ? variant<T, E, 128, 1, 64, 2>() : variant<T, E, 128, 2, 64, 2>();
-  return nb == 1 ? variant<T, E, 256, 1, 32, 2>() : variant<T, E, 256, 2, 32, 1>();
+  if (D == 64) return nb == 1 ? variant<T, E, 64, 1, 64, 4>() : variant<T, E, 64, 2, 64, 3>();
+  if (D == 128) return nb == 1 ? variant<T, E, 128, 1, 64, 3>() : variant<T, E, 128, 2, 64, 2>();
+  return nb == 1 ? variant<T, E, 256, 1, 32, 2>() : variant<T, E, 256, 2, 32, 2>();
 }
 
 // Shared memory granted to each variant, per device.
@@ -102,17 +105,29 @@ int attn(const dsa_kv_attn_args_t* a, void* stream) {
   std::atomic<bool>& granted = g_granted[dev][(c.D / 128) * 8 + (nb - 1) * 4 + (e ? 2 : 0) + (bf ? 1 : 0)];
   if (!granted.load(std::memory_order_relaxed)) {
     if (cudaFuncSetAttribute(reinterpret_cast<const void*>(v.fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)(v.smem + (kMaxCluster - 1) * v.more)) != cudaSuccess)
+                             (int)(kSmemPerSm - kSmemReserved)) != cudaSuccess)
       return DSA_KV_ERR_CUDA;
     granted.store(true, std::memory_order_relaxed);
   }
   // Few tiles: as many CTAs to each as stay resident at once, as long as every
-  // warp has a chunk. Measured (us with 1 / 2 / 4 / 8 CTAs per tile): 8 tiles of
-  // 32 chunks 15.6 / 11.3 / 9.4 / 8.9, 128 tiles of 64 chunks 34.4 / 27.2 / 32 /
-  // 43, 256 tiles of 128 chunks 91.5 / 96.3 / 105 / 136 (two CTAs fit an SM).
+  // warp has a chunk. Measured (us with 1 / 2 / 4 / 8 CTAs per tile; two fitted an
+  // SM): 8 tiles of 32 chunks 15.6 / 11.3 / 9.4 / 8.9, 128 tiles of 64 chunks
+  // 34.4 / 27.2 / 32 / 43, 256 tiles of 128 chunks 91.5 / 96.3 / 105 / 136.
   const int64_t resident = (int64_t)sms * v.ctas;
   int cluster = 1;
   while (cluster < kMaxCluster && tiles * cluster * 2 <= resident && items >= (int64_t)cluster * 2 * kAttnWarps) cluster *= 2;
+
+  // A grid of at most one wave spreads evenly over the SMs only if no more CTAs
+  // than its share fit one, because the next launch's are placed wherever the
+  // last ones of this leave room: shared memory is asked for until that is so
+  // (256 tiles of 8 heads, 8192 tokens: 87.0 instead of 96.0 us call after call).
+  const int64_t grid = tiles * cluster, per_sm = ceil_div(grid, sms);
+  const bool early = grid * 2 <= resident;
+  size_t smem = v.smem + (cluster - 1) * v.more;
+  if (!early && per_sm < v.ctas) {
+    const size_t least = kSmemPerSm / (per_sm + 1) - kSmemReserved + 1;  // one CTA more does not fit
+    if (smem < least) smem = least;
+  }
 
   AttnParams p;
   p.q = dense(a->q);
@@ -138,7 +153,7 @@ int attn(const dsa_kv_attn_args_t* a, void* stream) {
   p.K = (int32_t)a->K;
   p.bs = (int32_t)c.block_size;
   p.cluster = (uint32_t)cluster;
-  p.early = tiles * cluster * 2 <= resident;
+  p.early = early;
   p.log_pieces = log_pieces;
   p.box_bytes = (uint32_t)(box_rows * (c.D == 64 ? 64 : 128));
   p.block_bytes = bb;
@@ -150,7 +165,7 @@ int attn(const dsa_kv_attn_args_t* a, void* stream) {
                   !make_map(&v_map, c, c.v_codes, c.v_stride, box_rows)))
     return DSA_KV_ERR_CUDA;
 
-  return launch(v.fn, tiles * cluster, kAttnThreads, v.smem + (cluster - 1) * v.more, cluster, stream, p, k_map, v_map);
+  return launch(v.fn, grid, kAttnThreads, smem, cluster, stream, p, k_map, v_map);
 }
 
 }  // namespace kv

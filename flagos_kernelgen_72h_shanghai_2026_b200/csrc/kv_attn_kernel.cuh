@@ -31,17 +31,29 @@
 // instead, groups of up to 8 heads left half of every tile, and of the
 // exponentials and the output's registers, empty.
 //
-// Data movement: a chunk's key rows and value rows come by one TMA box each. A
-// warp has a ring of three boxes of its own, so that no CTA barrier is needed on
-// the way: the keys' box is refilled with the next chunk's values as soon as the
-// scores are done, the values' box with the keys of the chunk after that. Scales
-// follow by 4-byte asynchronous copies, and are turned into the token's factors
-// one chunk ahead. Rows are 128 bytes (64 for D = 64), swizzled by the copy,
-// which makes the 16-byte fragment reads free of bank conflicts: lane (g, c) of
-// a warp reads 32 contiguous bytes of key rows g and g + 8 for the products over
-// D, whose order of summation is free to choose, and 16 bytes of value rows 2c,
-// 2c+1, 2c+8, 2c+9 for the products over tokens, which are transposed pair by
-// pair with byte permutes. The weights change sides with movmatrix.
+// Data movement: a chunk's key rows and value rows come by one TMA box each, into
+// two boxes of the warp's own, so that no CTA barrier is needed on the way: the
+// keys' box is refilled as soon as the scores are done, the values' box after
+// the second product. Scales follow by 4-byte asynchronous copies. (A third box
+// a chunk ahead gained nothing, and took the third CTA's room. A producer warp
+// that starts all copies of a CTA was slower, 109 for 98 us: a TMA instruction
+// holds its warp for 85 cycles, and the rest of its work is one long chain.)
+// Rows are 128 bytes (64 for D = 64), swizzled by the copy, which makes the
+// 16-byte fragment reads free of bank conflicts: lane (g, c) of a warp reads 32
+// contiguous bytes of key rows g and g + 8 for the products over D, whose order
+// of summation is free to choose, and 16 bytes of value rows 2c, 2c+1, 2c+8,
+// 2c+9 for the products over tokens, which are transposed pair by pair with byte
+// permutes. The weights change sides with movmatrix.
+//
+// Why mma.sync: a row has at most 16 heads to multiply a key with, the least
+// tile of tcgen05 has 64 or 128 rows; with tokens as those rows the codes would
+// have to be written back to shared memory as fp16 first.
+//
+// What bounds it: a decode batch is bound by HBM (32 rows x 8 key heads over 8192
+// e4m3 tokens of D = 128: 87 us, 6.4 TB/s). Rows whose pages stay in L2 are bound
+// by what the warps issue: 290 cycles per SM for 32 tokens of 16 heads at
+// D = 128, of which the tensor pipe needs 128 and the conversion of codes (on the
+// half-rate integer pipe, with the byte permutes) 80.
 #pragma once
 
 #include <cuda.h>
@@ -89,14 +101,14 @@ struct AttnSmem {
   static constexpr int R = 8 * NB;                // query heads
   static constexpr size_t box = (size_t)TOK * D;  // keys or values of a chunk
   static constexpr size_t ring = 0;
-  static constexpr size_t region = 3 * box;       // of a warp; at the end its partial result
+  static constexpr size_t region = 2 * box;       // of a warp: keys, values; at the end its partial result
   static_assert((size_t)R * D * 4 <= region, "the ring holds the partial result");
-  static constexpr size_t tok = ring + W * region;                   // [W][2][TOK] factors of a chunk's tokens
-  static constexpr size_t scales = tok + (size_t)W * 2 * TOK * 16;   // [W][2][2][TOK]
-  static constexpr size_t bars = scales + (size_t)W * 2 * 2 * TOK * 4;  // [W][3]
-  static constexpr size_t ml = bars + (size_t)W * 3 * 8;             // [W][2][R] maxima and sums
+  static constexpr size_t tok = ring + W * region;                // [W][TOK] factors of a chunk's tokens
+  static constexpr size_t scales = tok + (size_t)W * TOK * 16;    // [W][2][TOK]
+  static constexpr size_t bars = scales + (size_t)W * 2 * TOK * 4;  // [W][2]
+  static constexpr size_t ml = bars + (size_t)W * 2 * 8;          // [W][2][R] maxima and sums
   static constexpr size_t fin = ml + (size_t)W * 2 * R * 4;          // [R] 1 / l
-  static constexpr bool q_in_smem = D == 256 && NB == 2;             // where the output fills the registers
+  static constexpr bool q_in_smem = D >= 128 && NB == 2;             // where the output fills the registers
   static constexpr size_t qf = fin + R * 4;
   static constexpr size_t all = qf + (q_in_smem ? (size_t)(D / 16) * NB * 32 * 8 : 0);
   // [C * W][R] weights of the cluster's warps
@@ -214,11 +226,11 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
 
   const uint32_t base = farq::smem_u32(smem);
   uint8_t* const ring = smem + L::ring + warp * L::region;
-  const uint32_t bars = base + (uint32_t)L::bars + warp * 3 * 8;
-  float* const scales = reinterpret_cast<float*>(smem + L::scales) + warp * 2 * 2 * TOK;
-  float4* const tok = reinterpret_cast<float4*>(smem + L::tok) + warp * 2 * TOK;
+  const uint32_t bars = base + (uint32_t)L::bars + warp * 2 * 8;
+  float* const scales = reinterpret_cast<float*>(smem + L::scales) + warp * 2 * TOK;
+  float4* const tok = reinterpret_cast<float4*>(smem + L::tok) + warp * TOK;
   if (lane == 0) {
-    for (int s = 0; s < 3; ++s) farq::mbar_init(bars + 8 * s, 1);
+    for (int s = 0; s < 2; ++s) farq::mbar_init(bars + 8 * s, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
@@ -327,7 +339,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     cp_page = __shfl_sync(0xffffffffu, pc_page, first + lane);
     cp_off = __shfl_sync(0xffffffffu, pc_off, first + lane);
   };
-  uint32_t started = 0;  // copies so far: the i-th fills box i % 3
+  uint32_t started = 0;  // copies so far: the i-th fills box i % 2
   auto copy = [&](const CUtensorMap* map, int s) {
     const uint32_t bar = bars + 8 * s;
     ++started;
@@ -340,11 +352,11 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     }
   };
   // Scales of this lane's tokens; zeros, and no access, where there are none.
-  auto copy_scales = [&](int buf) {
+  auto copy_scales = [&] {
 #pragma unroll
     for (int t = 0; t < LT; ++t) {
       const bool valid = (cp_mask[t] >> lane) & 1;
-      const uint32_t dst = farq::smem_u32(scales + buf * 2 * TOK + 32 * t + lane), bytes = valid ? 4 : 0;
+      const uint32_t dst = farq::smem_u32(scales + 32 * t + lane), bytes = valid ? 4 : 0;
       asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(valid ? cp_ks[t] : k_scale), "r"(bytes)
                    : "memory");
       asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + TOK * 4), "l"(valid ? cp_vs[t] : v_scale),
@@ -354,13 +366,13 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
   };
   // Factors of this lane's tokens: of their scores, the exponent and the
   // inverse of their value scales.
-  auto factors = [&](int buf) {
+  auto factors = [&] {
 #pragma unroll
     for (int t = 0; t < LT; ++t) {
-      const float ks = scales[buf * 2 * TOK + 32 * t + lane];
-      float vs = scales[buf * 2 * TOK + TOK + 32 * t + lane];
+      const float ks = scales[32 * t + lane];
+      float vs = scales[TOK + 32 * t + lane];
       vs = vs < kMinScale ? kMinScale : vs;
-      tok[buf * TOK + 32 * t + lane] = make_float4(ks * p.scale, __log2f(vs), rcp_approx(vs), 0.f);
+      tok[32 * t + lane] = make_float4(ks * p.scale, __log2f(vs), rcp_approx(vs), 0.f);
     }
   };
   // Rows that hold no token of the row: whatever lies there becomes zeros.
@@ -400,30 +412,20 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
   if (pos < 0) lim = 0;
   lim = min(lim, (int64_t)1 << 40);  // so that no product overflows
   look_up();
-  // The first chunk, and the second one's keys.
-  uint32_t issued = 0, mask[LT], next_mask[LT];
+  // The first chunk.
+  uint32_t mask[LT];
 #pragma unroll
-  for (int t = 0; t < LT; ++t) mask[t] = next_mask[t] = 0;
+  for (int t = 0; t < LT; ++t) mask[t] = 0;
   more = lim > 0;
   if (more) prepare();
-  if (more) {
+  bool have = more;  // a chunk to work on
+  if (have) {
     copy(&k_map, 0);
-    copy_scales(0);
+    copy_scales();
     copy(&v_map, 1);
-    ++issued;
 #pragma unroll
     for (int t = 0; t < LT; ++t) mask[t] = cp_mask[t];
   }
-  asm volatile("cp.async.commit_group;" ::: "memory");
-  if (more) prepare();
-  if (more) {
-    copy(&k_map, 2);
-    copy_scales(1);
-    ++issued;
-#pragma unroll
-    for (int t = 0; t < LT; ++t) next_mask[t] = cp_mask[t];
-  }
-  asm volatile("cp.async.commit_group;" ::: "memory");
 
   // In fp16, times the power of two that brings the CTA's largest finite value
   // into [2^14, 2^15).
@@ -486,19 +488,15 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
   }
   bool failed = false;
 
-  int s = 0;            // box of this chunk's keys; its values are in the next one
-  uint32_t parity = 0;  // of that box's copy
-  asm volatile("cp.async.wait_group 1;" ::: "memory");
-  if (issued > 0) factors(0);
-  __syncwarp();
-  for (uint32_t n = 0; n < issued; ++n) {
-    const float4* const now = tok + (n & 1) * TOK;
-    const int sv = s == 2 ? 0 : s + 1;
-    const uint32_t parity_v = s == 2 ? parity ^ 1 : parity;
-    uint8_t* const kbox = ring + s * L::box;
-    uint8_t* const vbox = ring + sv * L::box;
+  uint8_t* const kbox = ring;
+  uint8_t* const vbox = ring + L::box;
+  for (uint32_t parity = 0; have; parity ^= 1) {
+    // this chunk's factors, the next chunk's addresses
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    factors();
+    if (more) prepare();
     // a wait that runs out ends the loop before the next copy
-    failed = !farq::mbar_wait_bounded(bars + 8 * s, parity, kAttnWaitNs);
+    failed = !farq::mbar_wait_bounded(bars, parity, kAttnWaitNs);
     clear(kbox, mask);
 
     // scores: tile t has tokens 16t + g and 16t + g + 8 as this lane's rows
@@ -546,10 +544,12 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
           }
         }
       }
-    __syncwarp();  // the keys are read
+    __syncwarp();  // the keys and the scales are read, the factors written
     if (__any_sync(0xffffffffu, failed)) break;
-    if (n + 1 < issued) copy(&v_map, s);
-    if (more) prepare();
+    if (more) {
+      copy(&k_map, 0);
+      copy_scales();
+    }
 
     // exponents of heads 2c, 2c + 1 and tokens 8j + g. M moves when a lane
     // sees a value well above it; until then nothing has to be exchanged
@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     for (int t = 0; t < LT; ++t) partial |= mask[t] != 0xffffffffu;
 #pragma unroll
     for (int j = 0; j < 2 * NS; ++j) {
-      const float4 f = now[8 * j + g];
+      const float4 f = tok[8 * j + g];
       const float fx = f.x * qs;
       inv[j] = f.z;
 #pragma unroll
@@ -623,11 +623,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
         pw[j][x] = transpose8x8(Half16<__half>::pack(w0, w1));
       }
 
-    // the next chunk's factors
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    factors((n & 1) ^ 1);
-
-    failed |= !farq::mbar_wait_bounded(bars + 8 * sv, parity_v, kAttnWaitNs);
+    failed = !farq::mbar_wait_bounded(bars + 8, parity, kAttnWaitNs);
     clear(vbox, mask);
     // values times weights; rows g and g + 8 of output tile y are values
     // 16g + 2y and 16g + 2y + 1 of their box (8g + .. where D = 64)
@@ -664,25 +660,17 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
           }
       }
     }
-    __syncwarp();  // the values are read, the next factors are written
+    __syncwarp();  // the values and the factors are read
     if (__any_sync(0xffffffffu, failed)) break;
+    have = more;
+    if (more) copy(&v_map, 1);
 #pragma unroll
-    for (int t = 0; t < LT; ++t) mask[t] = next_mask[t];
-    if (more) {
-      copy(&k_map, sv);
-      copy_scales(n & 1);
-      ++issued;
-#pragma unroll
-      for (int t = 0; t < LT; ++t) next_mask[t] = cp_mask[t];
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    s = sv == 2 ? 0 : sv + 1;  // two boxes on
-    parity = sv == 2 ? parity_v ^ 1 : parity_v;
+    for (int t = 0; t < LT; ++t) mask[t] = cp_mask[t];
   }
   if (__any_sync(0xffffffffu, failed)) {
     // A copy did not arrive: wait (bounded) for those in flight, give NaN.
-    for (uint32_t i = started < 3 ? 0 : started - 3; i < started; ++i)
-      (void)farq::mbar_wait_bounded(bars + 8 * (i % 3), (i / 3) & 1, kAttnWaitNs);
+    for (uint32_t i = started < 2 ? 0 : started - 2; i < started; ++i)
+      (void)farq::mbar_wait_bounded(bars + 8 * (i % 2), (i / 2) & 1, kAttnWaitNs);
 #pragma unroll
     for (int x = 0; x < NB; ++x) l[x] = pair(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
   }
