@@ -432,20 +432,38 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
   uint32_t qf[QSMEM ? 1 : D / 16][NB][2];
   float qs;
   {
-    float most = 0.f;
+    // The largest magnitude is the largest of the bits without the sign; one
+    // that is not finite is left out, value by value.
+    uint32_t bits = 0;
 #pragma unroll
     for (int x = 0; x < NB; ++x)
 #pragma unroll
       for (int hh = 0; hh < NH; ++hh)
 #pragma unroll
         for (int i = 0; i < NU * 2; ++i) {
-          float f[8];
-          unpack8<T>(raw[x][hh][i], f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[e]) <= 3.4e38f ? fabsf(f[e]) : 0.f);
+          const uint4& v = raw[x][hh][i];
+          bits = __vmaxu2(bits, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
+                                         __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
         }
+    bits = max(bits & 0xffffu, bits >> 16);
+    bits = __reduce_max_sync(0xffffffffu, bits);
+    float most = Half16<T>::unpack(bits).x;
+    if (bits >= Half16<T>::kInf) {
+      most = 0.f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      for (int x = 0; x < NB; ++x)
+#pragma unroll
+        for (int hh = 0; hh < NH; ++hh)
+#pragma unroll
+          for (int i = 0; i < NU * 2; ++i) {
+            float f[8];
+            unpack8<T>(raw[x][hh][i], f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[e]) <= 3.4e38f ? fabsf(f[e]) : 0.f);
+          }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    }
     const int ex = max((int)(__float_as_uint(most) >> 23) - 127, -100);
     const float up = most > 0.f ? __uint_as_float((uint32_t)(14 - ex + 127) << 23) : 1.f;
     qs = 1.f / up;
@@ -725,7 +743,12 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
       const uint32_t n = sub + i * LPR;
       top[i] = -INFINITY;
       sum[i] = 0.f;
-      if (n < NW) {
+      if (C == 1) {
+        if (n < W) {
+          top[i] = ml[n * 2 * R + row];
+          sum[i] = ml[n * 2 * R + R + row];
+        }
+      } else if (n < NW) {
         const uint32_t at = mapa(base + (uint32_t)L::ml + ((n % W) * 2 * R + row) * 4, n / W);
         top[i] = ld_cluster(at);
         sum[i] = ld_cluster(at + R * 4);
@@ -753,7 +776,33 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     }
   }
   __syncthreads();
-  const int units = rows * (D / 4), share = (units + (int)C - 1) / (int)C;
+  auto store = [&](int row, int f4, const float4& acc) {
+    const float f = fin[row];
+    uint2 v;
+    v.x = Half16<T>::pack(acc.x * f, acc.y * f);
+    v.y = Half16<T>::pack(acc.z * f, acc.w * f);
+    *reinterpret_cast<uint2*>(p.out.row(b, qi, head0 + row) + f4 * 8) = v;
+  };
+  const int units = rows * (D / 4);
+  if (C == 1) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < units; i += kAttnThreads) {
+      const int row = i / (D / 4), f4 = i % (D / 4), at = part_index<D>(row, f4);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int n = 0; n < W; ++n) {
+        const float4 v = reinterpret_cast<const float4*>(smem + L::ring + n * L::region)[at];
+        const float w = all[n * R + row];
+        acc.x = fmaf(w, v.x, acc.x);
+        acc.y = fmaf(w, v.y, acc.y);
+        acc.z = fmaf(w, v.z, acc.z);
+        acc.w = fmaf(w, v.w, acc.w);
+      }
+      store(row, f4, acc);
+    }
+    return;
+  }
+  const int share = (units + (int)C - 1) / (int)C;
   int log_lanes = 0;
   while (log_lanes < 4 && (2u << log_lanes) <= NW && (share << (log_lanes + 1)) <= kAttnThreads) ++log_lanes;
   for (int i0 = 0; i0 < share; i0 += kAttnThreads >> log_lanes) {
@@ -777,15 +826,9 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
       acc.z += __shfl_xor_sync(0xffffffffu, acc.z, y);
       acc.w += __shfl_xor_sync(0xffffffffu, acc.w, y);
     }
-    if (mine && (threadIdx.x & ((1u << log_lanes) - 1)) == 0) {
-      const float f = fin[row];
-      uint2 v;
-      v.x = Half16<T>::pack(acc.x * f, acc.y * f);
-      v.y = Half16<T>::pack(acc.z * f, acc.w * f);
-      *reinterpret_cast<uint2*>(p.out.row(b, qi, head0 + row) + f4 * 8) = v;
-    }
+    if (mine && (threadIdx.x & ((1u << log_lanes) - 1)) == 0) store(row, f4, acc);
   }
-  if (C > 1) cluster_sync();  // shared memory stays until every CTA has read it
+  cluster_sync();  // shared memory stays until every CTA has read it
 }
 
 }  // namespace kv
