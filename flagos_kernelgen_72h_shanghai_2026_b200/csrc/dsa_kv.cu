@@ -113,7 +113,7 @@ int copy(const dsa_kv_copy_args_t* a, void* stream, bool write) {
   const int ib = index_size(a->pos_dtype), pb = index_size(a->page_dtype);
   if (!is_16bit(a->dtype) || !ib || !pb) return DSA_KV_ERR_BAD_DTYPE;
   if (a->B < 0 || a->Q < 0 || a->NB < 0) return DSA_KV_ERR_BAD_SHAPE;
-  int st = check_cache(a->cache, write);
+  int st = check_cache(a->cache, write ? kCacheWritten : kCacheRead);
   if (st != DSA_KV_OK) return st;
   const dsa_kv_cache_t& c = a->cache;
   if (!fits(a->B, a->Q, 2 * c.H) || a->NB > kMaxIndex) return DSA_KV_ERR_UNSUPPORTED;

@@ -66,7 +66,7 @@ int attn(const dsa_kv_attn_args_t* a, void* stream) {
   const int bb = index_size(a->block_dtype), pb = index_size(a->page_dtype), ib = index_size(a->pos_dtype);
   if (!is_16bit(a->dtype) || !bb || !pb || !ib) return DSA_KV_ERR_BAD_DTYPE;
   if (a->B < 0 || a->Q < 0 || a->G < 1 || a->K < 0) return DSA_KV_ERR_BAD_SHAPE;
-  int st = check_cache(a->cache, false);
+  int st = check_cache(a->cache, kCacheMapped);
   if (st != DSA_KV_OK) return st;
   const dsa_kv_cache_t& c = a->cache;
   if ((c.D != 64 && c.D != 128 && c.D != 256) || c.block_size < 8) return DSA_KV_ERR_BAD_HEAD_DIM;

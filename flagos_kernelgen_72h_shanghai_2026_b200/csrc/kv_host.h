@@ -48,7 +48,10 @@ inline Dense dense(const dsa_kv_dense_t& t) {
   return d;
 }
 
-inline int check_cache(const dsa_kv_cache_t& c, bool written) {
+// Uses of a cache: scales (and, read by plain loads, codes) may be broadcast by
+// strides of 0; what is written may not, and tensor maps take codes as they lie.
+enum CacheUse { kCacheRead, kCacheWritten, kCacheMapped };
+inline int check_cache(const dsa_kv_cache_t& c, CacheUse use) {
   if (c.reserved0 != 0) return DSA_KV_ERR_BAD_ARGS_SIZE;
   if (c.code_dtype != DSA_KV_INT8 && c.code_dtype != DSA_KV_E4M3) return DSA_KV_ERR_BAD_DTYPE;
   if (c.P < 0 || c.H < 1 || c.block_size < 1) return DSA_KV_ERR_BAD_SHAPE;
@@ -62,10 +65,12 @@ inline int check_cache(const dsa_kv_cache_t& c, bool written) {
   for (int i = 0; i < 3; ++i) {
     if (n[i] <= 1) continue;
     if (c.k_stride[i] % 16 != 0 || c.v_stride[i] % 16 != 0) return DSA_KV_ERR_ALIGNMENT;
-    const int64_t least = written ? 1 : 0;
-    if (c.k_stride[i] < least || c.v_stride[i] < least || c.k_scale_stride[i] < least ||
-        c.v_scale_stride[i] < least)
+    const int64_t least = use == kCacheRead ? 0 : 1, least_scale = use == kCacheWritten ? 1 : 0;
+    if (c.k_stride[i] < least || c.v_stride[i] < least || c.k_scale_stride[i] < least_scale ||
+        c.v_scale_stride[i] < least_scale)
       return DSA_KV_ERR_BAD_SHAPE;
+    if (use == kCacheMapped && (c.k_stride[i] >= (int64_t)1 << 40 || c.v_stride[i] >= (int64_t)1 << 40))
+      return DSA_KV_ERR_UNSUPPORTED;
   }
   return DSA_KV_OK;
 }

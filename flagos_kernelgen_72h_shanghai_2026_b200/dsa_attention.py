@@ -36,9 +36,10 @@ def dsa_paged_attention(q: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.T
     """out = softmax(softmax_scale * q k^T) v over each row's selected tokens; returns ``(out, lse)``.
 
     q, out [B, Q, Hq, D] bf16 or fp16 (strided views whose rows start on 16
-    bytes); Hq is a multiple of the cache's H, query heads h * Hq/H and on
+    bytes; out may be q itself); Hq is a multiple of the cache's H, query heads h * Hq/H and on
     share key head h and its selection. The cache as in ``kv_cache``: codes
-    [P, H, block_size, D], scales [P, H, block_size]. blocks, pages
+    [P, H, block_size, D], scales [P, H, block_size], which may be broadcast
+    (one scale per head, or for all). blocks, pages
     [B, H, Q, K] int32 or int64 (the last dimension contiguous; the others may
     be broadcast): entry i stands for the tokens t of block ``blocks[..., i]``,
     stored in page ``pages[..., i]``, with t <= q_pos[b, q] and t < kv_lens[b].

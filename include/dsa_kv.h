@@ -75,7 +75,9 @@ typedef struct dsa_kv_dense {
  * holds a NaN or an infinity gets the scale NaN and the codes 0, so that it
  * reads back as NaN.
  * Strides: codes in elements (bytes), scales in floats; D is contiguous, code
- * rows start on 16 bytes.
+ * rows start on 16 bytes. A read and the attention take scales broadcast by
+ * strides of 0 (one scale per head, or for all); the attention's strides are
+ * below 2^40 (codes) and 2^31 (scales).
  */
 typedef struct dsa_kv_cache {
     int32_t code_dtype;           /* INT8 | E4M3                                   */
@@ -152,6 +154,7 @@ typedef struct dsa_kv_copy_args {
  * counts twice.
  *     out = sum_t softmax(scale * q.k_t) v_t,   lse = ln sum_t exp(scale * q.k_t)
  * A row without a token (and a padded one, q_pos < 0) has out = 0, lse = -inf.
+ * out may be q itself.
  * v_scale is positive; one below 1e-12, the least that a write leaves, counts
  * as 1e-12.
  * D is 64, 128 or 256, block_size >= 8.

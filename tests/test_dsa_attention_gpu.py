@@ -15,7 +15,10 @@ them, n tokens, D the head size):
 """
 import ctypes
 import math
+import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import pytest
 import torch
@@ -269,6 +272,65 @@ def test_broadcast_selection_is_dense_attention(dev):
     out, lse = torch.empty_like(q, device=dev), torch.empty(2, 5, 8, device=dev)
     dsa_paged_attention(q.to(dev), *cd, bd, pd, pos.to(dev), lens.to(dev), out, lse, 0.1)
     check(out, lse, r, 128, 448.0)
+
+
+def test_broadcast_scales(dev):
+    """One scale per head, and one for all keys, by strides of 0."""
+    _, _, P, c, q, blocks, pages, pos, lens = inputs(44)
+    c[1], c[3] = torch.tensor(0.01).expand(P, 2, 32), torch.tensor([0.02, 0.5])[:, None].expand(P, 2, 32)
+    r = R.dsa_paged_attention_ref(q, *c, blocks, pages, pos, lens, 0.1)
+    cd = [c[0].to(dev), torch.tensor(0.01, device=dev).expand(P, 2, 32), c[2].to(dev),
+          torch.tensor([0.02, 0.5], device=dev)[:, None].expand(P, 2, 32)]
+    out, lse = torch.empty_like(q, device=dev), torch.empty(q.shape[:3], device=dev)
+    dsa_paged_attention(q.to(dev), *cd, *(t.to(dev) for t in (blocks, pages, pos, lens)), out, lse, 0.1)
+    check(out, lse, r, 128, 448.0)
+
+
+@pytest.mark.parametrize("B,Q,K", [(1, 1, 8), (8, 16, 8)])
+def test_in_place(dev, B, Q, K):
+    """The output over the queries, with clusters (few rows) and without."""
+    _, _, _, c, q, blocks, pages, pos, lens = inputs(45, B=B, Q=Q, K=K, G=16)
+    want, lse = run(dev, q, c, blocks, pages, pos, lens, 0.1)
+    qd = q.to(dev)
+    got = dsa_paged_attention(qd, *(t.to(dev) for t in (*c, blocks, pages, pos, lens)), qd, None, 0.1)
+    assert got[0] is qd and torch.equal(qd, want)
+
+
+_FIRST_IN_CAPTURE = """
+import torch
+from flagos_kernelgen_72h_shanghai_2026_b200 import *
+dev = torch.device("cuda:0")
+q = torch.randn(1, 2, 4, 64, device=dev).half()
+k, v = torch.randn(1, 2, 2, 64, device=dev).half(), torch.randn(1, 2, 2, 64, device=dev).half()
+gamma, pos = torch.ones(64, device=dev), torch.arange(2, dtype=torch.int32, device=dev)[None]
+cs = torch.cat([torch.ones(8, 32), torch.zeros(8, 32)], 1).to(dev)
+cache = (torch.zeros(3, 2, 16, 64, dtype=torch.int8, device=dev), torch.zeros(3, 2, 16, device=dev),
+         torch.zeros(3, 2, 16, 64, dtype=torch.int8, device=dev), torch.zeros(3, 2, 16, device=dev))
+table, lens = torch.tensor([[2, 0]], dtype=torch.int32, device=dev), torch.tensor([2], dtype=torch.int32, device=dev)
+sel, pages = torch.zeros(1, 2, 2, 1, dtype=torch.int32, device=dev), torch.full((1, 2, 2, 1), 2, dtype=torch.int32, device=dev)
+qo, ko, out, k2, v2 = (torch.zeros_like(t) for t in (q, k, q, k, v))
+side = torch.cuda.Stream()
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=side):
+    qk_rmsnorm_rope(q, k, gamma, gamma, cs, pos, qo, ko, 1e-6)
+    paged_kv_quant_write(ko, v, *cache, table, pos)
+    dsa_paged_attention(qo, *cache, sel, pages, pos, lens, out, None, 0.125)
+    paged_kv_dequant_read(*cache, table, lens, k2, v2)
+g.replay()
+torch.cuda.synchronize()
+n = q.float() / (q.float().square().mean(-1, keepdim=True) + 1e-6).sqrt()
+assert (qo.float() - n).abs().max() < 0.01 and (k2 - ko).abs().max() < 0.03 and (v2 - v).abs().max() < 0.03
+assert (out[0, 0].view(2, 2, 64) - v2[0, 0][:, None]).abs().max() < 0.01  # the first token sees itself alone
+print("captured")
+"""
+
+
+def test_first_calls_of_a_process_in_a_capture(dev):
+    """Nothing was launched, loaded or set up before the capture begins."""
+    p = subprocess.run([sys.executable, "-c", _FIRST_IN_CAPTURE], capture_output=True, text=True, timeout=300,
+                       cwd=Path(__file__).resolve().parent.parent)
+    assert p.returncode == 0 and "captured" in p.stdout, p.stderr[-2000:]
 
 
 def test_strided_queries_and_outputs(dev):

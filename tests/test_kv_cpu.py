@@ -115,6 +115,10 @@ def _attn(**kw):
     (dict(pages=0x80004), L.ERR_ALIGNMENT),
     (dict(lse=0xb0002), L.ERR_ALIGNMENT),
     (dict(cache__v_codes=0x40004), L.ERR_ALIGNMENT),
+    (dict(cache__k_stride=(4096, 0, 128)), L.ERR_BAD_SHAPE),
+    (dict(cache__v_stride=(1 << 40, 2048, 128)), L.ERR_UNSUPPORTED),
+    (dict(cache__v_scale_stride=(1 << 31, 16, 1)), L.ERR_UNSUPPORTED),
+    (dict(cache__k_scale_stride=(-16, 16, 1)), L.ERR_BAD_SHAPE),
 ])
 def test_attention_validation_before_any_device_call(lib, kw, code):
     assert lib.dsa_kv_attn_launch(ctypes.byref(_attn(**kw)), None) == code
