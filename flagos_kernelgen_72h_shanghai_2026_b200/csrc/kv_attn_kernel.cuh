@@ -38,12 +38,11 @@
 // a chunk ahead gained nothing, and took the third CTA's room. A producer warp
 // that starts all copies of a CTA was slower, 109 for 98 us: a TMA instruction
 // holds its warp for 85 cycles, and the rest of its work is one long chain.)
-// Rows are 128 bytes (64 for D = 64), swizzled by the copy, which makes the
-// 16-byte fragment reads free of bank conflicts: lane (g, c) of a warp reads 32
-// contiguous bytes of key rows g and g + 8 for the products over D, whose order
-// of summation is free to choose, and 16 bytes of value rows 2c, 2c+1, 2c+8,
-// 2c+9 for the products over tokens, which are transposed pair by pair with byte
-// permutes. The weights change sides with movmatrix.
+// Rows are 128 bytes (64 for D = 64), swizzled by the copy, which makes all
+// fragment reads free of bank conflicts: a lane reads 32 contiguous bytes of two
+// key rows of a tile for the products over D, whose order of summation is free
+// to choose; value tiles come transposed, byte by byte, through ldmatrix. The
+// weights change sides with movmatrix.
 //
 // Why mma.sync: a row has at most 16 heads to multiply a key with, the least
 // tile of tcgen05 has 64 or 128 rows; with tokens as those rows the codes would
@@ -52,8 +51,8 @@
 // What bounds it: a decode batch is bound by HBM (32 rows x 8 key heads over 8192
 // e4m3 tokens of D = 128: 87 us, 6.4 TB/s). Rows whose pages stay in L2 are bound
 // by what the warps issue: 290 cycles per SM for 32 tokens of 16 heads at
-// D = 128, of which the tensor pipe needs 128 and the conversion of codes (on the
-// half-rate integer pipe, with the byte permutes) 80.
+// D = 128, of which the tensor pipe needs 128 and the conversion of codes, on the
+// half-rate integer pipe, 64.
 #pragma once
 
 #include <cuda.h>
@@ -131,6 +130,27 @@ __device__ __forceinline__ void mma16816(float c[4], const uint32_t a[4], uint32
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// c = a * b.
+__device__ __forceinline__ void mma16816_first(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9},"
+      " {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+// Two 16 x 16 tiles of bytes, transposed: row addresses from lanes 0 to 15 and
+// 16 to 31. Lane (g, c) gets rows 4c to 4c + 3 of column g (r[0], r[2]) and of
+// column g + 8 (r[1], r[3]).
+__device__ __forceinline__ void load_transposed(uint32_t r[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -193,11 +213,10 @@ __device__ __forceinline__ void cluster_sync() {
 }
 
 // Place of float4 `f4` of head `row` in a warp's partial result: the units of a
-// head are permuted so that the writes of a quarter warp spread over the banks.
+// head are permuted so that the lanes' writes spread over the banks.
 template <int D>
 __device__ __forceinline__ int part_index(int row, int f4) {
-  const int c = (row >> 1) & 3;
-  return row * (D / 4) + (f4 ^ (D == 64 ? (c & 1) | ((c >> 1) << 2) : c));
+  return row * (D / 4) + (f4 ^ (((row >> 1) & 3) << 1));
 }
 
 template <typename T, int D, bool E4M3, int NB, int TOK, int CTAS>
@@ -364,6 +383,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
                    : "memory");
     }
   };
+  float qs = 0.f;  // softmax_scale * log2(e) over the factor of the queries
   // Factors of this lane's tokens: of their scores, the exponent and the
   // inverse of their value scales.
   auto factors = [&] {
@@ -372,7 +392,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
       const float ks = scales[32 * t + lane];
       float vs = scales[TOK + 32 * t + lane];
       vs = vs < kMinScale ? kMinScale : vs;
-      tok[32 * t + lane] = make_float4(ks * p.scale, __log2f(vs), rcp_approx(vs), 0.f);
+      tok[32 * t + lane] = make_float4(ks * qs, __log2f(vs), rcp_approx(vs), 0.f);
     }
   };
   // Rows that hold no token of the row: whatever lies there becomes zeros.
@@ -430,7 +450,6 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
   // In fp16, times the power of two that brings the CTA's largest finite value
   // into [2^14, 2^15).
   uint32_t qf[QSMEM ? 1 : D / 16][NB][2];
-  float qs;
   {
     // The largest magnitude is the largest of the bits without the sign; one
     // that is not finite is left out, value by value.
@@ -466,7 +485,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     }
     const int ex = max((int)(__float_as_uint(most) >> 23) - 127, -100);
     const float up = most > 0.f ? __uint_as_float((uint32_t)(14 - ex + 127) << 23) : 1.f;
-    qs = 1.f / up;
+    qs = p.scale / up;
 #pragma unroll
     for (int x = 0; x < NB; ++x)
 #pragma unroll
@@ -506,6 +525,13 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
   }
   bool failed = false;
 
+  // Row r of a 16-row tile is token 4 (r / 2) + r % 2 for r < 8, two further for
+  // r + 8: so the weights come out in the order of the transposed values, of
+  // which a lane gets four tokens in a row.
+  const int g0 = 4 * (g >> 1) + (g & 1);
+  const int vr = lane & 15;  // this lane's row of a tile of values, and its 16-byte unit
+  const uint32_t vaddr = farq::smem_u32(ring) + (uint32_t)L::box + vr * ROWB +
+                         (((lane >> 4) ^ (D == 64 ? (vr >> 1) & 3 : vr & 7)) << 4);
   uint8_t* const kbox = ring;
   uint8_t* const vbox = ring + L::box;
   for (uint32_t parity = 0; have; parity ^= 1) {
@@ -517,23 +543,18 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     failed = !farq::mbar_wait_bounded(bars, parity, kAttnWaitNs);
     clear(kbox, mask);
 
-    // scores: tile t has tokens 16t + g and 16t + g + 8 as this lane's rows
+    // scores of tiles of 16 tokens
     float sc[NS][NB][4];
-#pragma unroll
-    for (int t = 0; t < NS; ++t)
-#pragma unroll
-      for (int x = 0; x < NB; ++x)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sc[t][x][e] = 0.f;
 #pragma unroll
     for (int hh = 0; hh < NH; ++hh)
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
-        uint4 kw[2 * NS];  // key rows 8j + g
+        uint4 kw[2 * NS];  // key rows, two of each tile
 #pragma unroll
         for (int j = 0; j < 2 * NS; ++j) {
-          const uint32_t at = D == 64 ? (8 * j + g) * 64 + ((c ^ ((g >> 1) & 3)) << 4)
-                                      : hh * TOK * 128 + (8 * j + g) * 128 + (((2 * c + u) ^ g) << 4);
+          const int row = 16 * (j >> 1) + 2 * (j & 1) + g0;
+          const uint32_t at = D == 64 ? row * 64 + ((c ^ ((row >> 1) & 3)) << 4)
+                                      : hh * TOK * 128 + row * 128 + (((2 * c + u) ^ (row & 7)) << 4);
           kw[j] = *reinterpret_cast<const uint4*>(kbox + at);
         }
 #pragma unroll
@@ -558,7 +579,12 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
             decode_pairs<E4M3>(i == 0 ? lo.x : i == 1 ? lo.y : i == 2 ? lo.z : lo.w, a[0], a[2]);
             decode_pairs<E4M3>(i == 0 ? hi.x : i == 1 ? hi.y : i == 2 ? hi.z : hi.w, a[1], a[3]);
 #pragma unroll
-            for (int x = 0; x < NB; ++x) mma16816(sc[t][x], a, bq[x][0], bq[x][1]);
+            for (int x = 0; x < NB; ++x) {
+              if (hh + u + i == 0)
+                mma16816_first(sc[t][x], a, bq[x][0], bq[x][1]);
+              else
+                mma16816(sc[t][x], a, bq[x][0], bq[x][1]);
+            }
           }
         }
       }
@@ -569,40 +595,37 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
       copy_scales();
     }
 
-    // exponents of heads 2c, 2c + 1 and tokens 8j + g. M moves when a lane
-    // sees a value well above it; until then nothing has to be exchanged
-    // between lanes.
+    // exponents of heads 2c, 2c + 1. M moves when a lane sees a value well above
+    // it; until then nothing has to be exchanged between lanes.
     f32x2 a[2 * NS][NB];
     float inv[2 * NS], m[NB][2];
-#pragma unroll
-    for (int x = 0; x < NB; ++x) m[x][0] = m[x][1] = -INFINITY;
     bool partial = false;
 #pragma unroll
     for (int t = 0; t < LT; ++t) partial |= mask[t] != 0xffffffffu;
 #pragma unroll
     for (int j = 0; j < 2 * NS; ++j) {
-      const float4 f = tok[8 * j + g];
-      const float fx = f.x * qs;
+      const float4 f = tok[16 * (j >> 1) + 2 * (j & 1) + g0];
       inv[j] = f.z;
 #pragma unroll
       for (int x = 0; x < NB; ++x)
-        a[j][x] = fma2(pair(sc[j >> 1][x][(j & 1) * 2], sc[j >> 1][x][(j & 1) * 2 + 1]), pair(fx, fx), pair(f.y, f.y));
+        a[j][x] = fma2(pair(sc[j >> 1][x][(j & 1) * 2], sc[j >> 1][x][(j & 1) * 2 + 1]), pair(f.x, f.x), pair(f.y, f.y));
     }
     if (partial) {
 #pragma unroll
       for (int j = 0; j < 2 * NS; ++j)
 #pragma unroll
         for (int x = 0; x < NB; ++x)
-          if (!((mask[j / 4] >> (8 * (j & 3) + g)) & 1)) a[j][x] = pair(-INFINITY, -INFINITY);
+          if (!((mask[j / 4] >> (16 * ((j >> 1) & 1) + 2 * (j & 1) + g0)) & 1)) a[j][x] = pair(-INFINITY, -INFINITY);
     }
     bool moves = false;
 #pragma unroll
     for (int x = 0; x < NB; ++x) {
+      m[x][0] = m[x][1] = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 2 * NS; ++j) {
-        const float2 v = both(a[j][x]);
-        m[x][0] = fmaxf(m[x][0], v.x);
-        m[x][1] = fmaxf(m[x][1], v.y);
+      for (int j = 0; j < 2 * NS; j += 2) {
+        const float2 v = both(a[j][x]), w = both(a[j + 1][x]);
+        m[x][0] = max3(m[x][0], v.x, w.x);
+        m[x][1] = max3(m[x][1], v.y, w.y);
       }
       moves |= m[x][0] > M[x][0] + kLag || m[x][1] > M[x][1] + kLag;
     }
@@ -629,7 +652,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
         }
       }
     }
-    // weights, as the columns of the second product: tokens 2c, 2c + 1 of head g
+    // weights, as the columns of the second product: rows 2c, 2c + 1 of head g
     uint32_t pw[2 * NS][NB];
 #pragma unroll
     for (int x = 0; x < NB; ++x)
@@ -643,41 +666,24 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
 
     failed = !farq::mbar_wait_bounded(bars + 8, parity, kAttnWaitNs);
     clear(vbox, mask);
-    // values times weights; rows g and g + 8 of output tile y are values
-    // 16g + 2y and 16g + 2y + 1 of their box (8g + .. where D = 64)
+    // values times weights: rows g and g + 8 of output tile y are values 16y + g and 16y + g + 8
 #pragma unroll
-    for (int t = 0; t < NS; ++t) {
+    for (int t = 0; t < NS; ++t)
 #pragma unroll
-      for (int hh = 0; hh < NH; ++hh) {
-        constexpr int NWORD = D == 64 ? 2 : 4;
-        uint32_t w[4][NWORD];
+      for (int hh = 0; hh < NH; ++hh)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int row = 16 * t + 2 * c + (x & 1) + 8 * (x >> 1);
-          if constexpr (D == 64) {
-            const uint2 v = *reinterpret_cast<const uint2*>(vbox + row * 64 + (((g >> 1) ^ c) << 4) + (g & 1) * 8);
-            w[x][0] = v.x;
-            w[x][1] = v.y;
-          } else {
-            const uint4 v = *reinterpret_cast<const uint4*>(vbox + hh * TOK * 128 + row * 128 + ((g ^ (2 * c + (x & 1))) << 4));
-            w[x][0] = v.x;
-            w[x][1] = v.y;
-            w[x][2] = v.z;
-            w[x][3] = v.w;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < NWORD; ++i)
+        for (int y = 0; y < NT / NH; y += 2) {
+          uint32_t w[4];
+          load_transposed(w, (vaddr + t * 16 * ROWB + hh * TOK * 128) ^ (y << 4));
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             uint32_t a[4];
-            decode_pairs<E4M3>(__byte_perm(w[0][i], w[1][i], e ? 0x7362 : 0x5140), a[0], a[1]);
-            decode_pairs<E4M3>(__byte_perm(w[2][i], w[3][i], e ? 0x7362 : 0x5140), a[2], a[3]);
+            decode_pairs<E4M3>(w[2 * e], a[0], a[2]);
+            decode_pairs<E4M3>(w[2 * e + 1], a[1], a[3]);
 #pragma unroll
-            for (int x = 0; x < NB; ++x) mma16816(o[hh * 8 + 2 * i + e][x], a, pw[2 * t][x], pw[2 * t + 1][x]);
+            for (int x = 0; x < NB; ++x) mma16816(o[hh * 8 + y + e][x], a, pw[2 * t][x], pw[2 * t + 1][x]);
           }
-      }
-    }
+        }
     __syncwarp();  // the values and the factors are read
     if (__any_sync(0xffffffffu, failed)) break;
     have = more;
@@ -698,7 +704,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
 
   // Partial results into the warp's own ring, whose copies are all done.
   float* const ml = reinterpret_cast<float*>(smem + L::ml);
-  float4* const part = reinterpret_cast<float4*>(smem + L::ring + (size_t)warp * L::region);
+  float* const part = reinterpret_cast<float*>(smem + L::ring + (size_t)warp * L::region);
 #pragma unroll
   for (int x = 0; x < NB; ++x)
 #pragma unroll
@@ -712,13 +718,9 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
         ml[warp * 2 * R + R + row] = sum;
       }
 #pragma unroll
-      for (int hh = 0; hh < NH; ++hh) {
-        constexpr int RUN = NT / NH;  // tiles of a box: 8, or 4 where D = 64
-#pragma unroll
-        for (int i = 0; i < RUN; i += 2) {
-          const int f4 = (hh * 128 + g * 2 * RUN + 2 * i) / 4, t = hh * 8 + i;
-          part[part_index<D>(row, f4)] = make_float4(o[t][x][e], o[t][x][2 + e], o[t + 1][x][e], o[t + 1][x][2 + e]);
-        }
+      for (int y = 0; y < NT; ++y) {
+        part[row * D + ((16 * y + g) ^ (c << 3))] = o[y][x][e];
+        part[row * D + ((16 * y + 8 + g) ^ (c << 3))] = o[y][x][2 + e];
       }
     }
   if (C > 1)
