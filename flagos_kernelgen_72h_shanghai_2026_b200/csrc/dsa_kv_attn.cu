@@ -47,7 +47,7 @@ Variant variant() {
 // (us): chunks of 64 tokens against 32 with 16 heads at D = 128, 1024 rows x
 // 2048 tokens: 95.7 against 108.5 (three CTAs of 32) and 118 (two): what a chunk
 // costs besides its products weighs more than the warps that hide it. Three
-// CTAs against two there: 100.4 against 94.9; with 8 heads, 2048 rows: 116
+// CTAs against two there: 102 against 88.0; with 8 heads, 2048 rows: 116
 // against 134; at D = 64, 2048 rows: 74 (four) against 81 (three) with 8 heads,
 // 104 (three) against 122 (two) with 16.
 template <typename T, bool E>

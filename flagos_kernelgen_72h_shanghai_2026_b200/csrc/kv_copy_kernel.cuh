@@ -10,8 +10,8 @@
 // worked out once for the 2U vectors that a lane then moves: with one vector
 // per look-up the kernels were bound by that arithmetic (170 instructions for
 // two vectors of a read, 75 % of the issue slots at 3.8 TB/s). Read of 8 x up to
-// 8192 tokens x 8 heads x 128 (e4m3 to bf16): 53.8 us, 5.9 TB/s; write of
-// 2 x 4096 tokens: 10.9 us, 4.2 TB/s.
+// 8192 tokens x 8 heads x 128 (e4m3 to bf16): 52.8 us, 6.0 TB/s; write of
+// 2 x 4096 tokens: 11.0 us, 4.2 TB/s.
 #pragma once
 
 #include "kv_common.cuh"

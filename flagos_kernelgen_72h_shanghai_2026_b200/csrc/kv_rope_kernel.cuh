@@ -11,13 +11,14 @@
 // 8 values is another lane's 8 values, fetched as four packed words by
 // shuffles; adjacent pairs lie within the lane. Gamma, cosine and sine are
 // multiplied into two factors for each value, once for a token's queries and
-// once for its keys: 75 instead of 180 instructions for a warp's two heads of
-// 128, which had bound the kernel (62 % of the issue slots).
+// once for its keys: 123 instead of 181 instructions in all for a warp's two
+// heads of 128, which had bound the kernel.
 //
-// 8192 tokens x 40 heads x 128, bf16: 32.8 us, 5.2 TB/s. One warp per 16 heads
-// and token, without the next step's loads in flight, took 38.3 us: the chain
-// position, angles, values was waited for in every CTA (19 warps per SM active,
-// most of them on loads). What is left is the same wait at a smaller scale.
+// 8192 tokens x 40 heads x 128, bf16: 34.0 us, 5.1 TB/s, 62 % of the issue
+// slots. One warp per 16 heads and token, without the next step's loads in
+// flight, took 38.3 us: the chain position, angles, values was waited for in
+// every CTA (19 warps per SM active, most of them on loads). What is left is
+// the same wait at a smaller scale.
 #pragma once
 
 #include "kv_common.cuh"
