@@ -49,9 +49,12 @@ struct CacheSide {
   int64_t ssp, ssh, sst;
 };
 
+// No load of these kernels is of the read-only kind (ld.global.nc): a grid that
+// was launched early is already running while the one before it writes what
+// it will read.
 __device__ __forceinline__ int64_t load_index(const void* p, int64_t i, int bytes) {
-  return bytes == 8 ? (int64_t)__ldg(reinterpret_cast<const long long*>(p) + i)
-                    : (int64_t)__ldg(reinterpret_cast<const int*>(p) + i);
+  return bytes == 8 ? (int64_t)reinterpret_cast<const long long*>(p)[i]
+                    : (int64_t)reinterpret_cast<const int*>(p)[i];
 }
 
 // Programmatic dependent launch: the grid may start while the previous kernel

@@ -160,8 +160,8 @@ __global__ void __launch_bounds__(kCopyThreads) read_kernel(const CopyParams p) 
       if (cell && w.h + u * hps < p.H) {
         codes[u] = ld_stream8(ks + (int64_t)(u * hps) * p.kc.sh);
         codes[U + u] = ld_stream8(vs + (int64_t)(u * hps) * p.vc.sh);
-        scale[u] = __ldg(kf + (int64_t)(u * hps) * p.kc.ssh);
-        scale[U + u] = __ldg(vf + (int64_t)(u * hps) * p.vc.ssh);
+        scale[u] = kf[(int64_t)(u * hps) * p.kc.ssh];
+        scale[U + u] = vf[(int64_t)(u * hps) * p.vc.ssh];
       }
     }
   }

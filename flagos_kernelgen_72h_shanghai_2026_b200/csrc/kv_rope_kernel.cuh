@@ -48,11 +48,11 @@ struct RopeParams {
 __device__ __forceinline__ void load_gamma8(const void* g, int i, int dtype, float f[8]) {
   if (dtype == DSA_KV_FP32) {
     const float4* p = reinterpret_cast<const float4*>(g) + 2 * i;
-    const float4 a = __ldg(p), b = __ldg(p + 1);
+    const float4 a = p[0], b = p[1];
     f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
     f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
   } else {
-    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(g) + i);
+    const uint4 raw = reinterpret_cast<const uint4*>(g)[i];
     if (dtype == DSA_KV_BF16)
       unpack8<__nv_bfloat16>(raw, f);
     else
@@ -103,8 +103,8 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeCtas) rope_kernel(const Rop
     const float* row = p.cos_sin + at * p.rot + (INTERLEAVED ? 4 * i : 8 * (i < hl ? i : i - hl));
 #pragma unroll
     for (int e = 0; e < NA; e += 4) {
-      const float4 c = __ldg(reinterpret_cast<const float4*>(row + e));
-      const float4 s = __ldg(reinterpret_cast<const float4*>(row + (p.rot >> 1) + e));
+      const float4 c = *reinterpret_cast<const float4*>(row + e);
+      const float4 s = *reinterpret_cast<const float4*>(row + (p.rot >> 1) + e);
       cs[e] = c.x; cs[e + 1] = c.y; cs[e + 2] = c.z; cs[e + 3] = c.w;
       sn[e] = s.x; sn[e + 1] = s.y; sn[e + 2] = s.z; sn[e + 3] = s.w;
     }

@@ -1,6 +1,6 @@
 """Plain implementations in 64 bits of the operators around the paged KV cache
-(TEST INFRASTRUCTURE: only tests/ and __graft_entry__.smoke() use this module,
-as the checker; the product path never imports it).
+(TEST INFRASTRUCTURE: only tests/ and __graft_entry__.smoke() use this module;
+the product path never imports it).
 
 Everything is computed on the CPU in float64 from the operators' formulas
 (include/dsa_kv.h), token by token where that says more than a batched form.
