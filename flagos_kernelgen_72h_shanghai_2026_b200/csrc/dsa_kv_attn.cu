@@ -60,6 +60,32 @@ Variant variant_of(int64_t D, int nb) {
 // Shared memory granted to each variant, per device.
 std::atomic<bool> g_granted[kMaxDevices][24];
 
+// Clusters of 2^log_c CTAs that are resident at once with up to n of their CTAs
+// on an SM: less than the SMs' number gives, as a cluster stays within one group
+// of SMs. With shared memory for no more than n, it does not depend on the variant.
+int64_t max_clusters(const Variant& v, int dev, int n, int log_c) {
+  static std::atomic<int> known[kMaxDevices][8][4];  // plus one
+  std::atomic<int>& have = known[dev][n - 1][log_c];
+  int count = have.load(std::memory_order_relaxed) - 1;
+  if (count >= 0) return count;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 1u << log_c;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(1u << log_c);
+  cfg.blockDim = dim3(kAttnThreads);
+  cfg.dynamicSmemBytes = kSmemPerSm / n - kSmemReserved;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&count, reinterpret_cast<const void*>(v.fn), &cfg) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 0;  // no clusters then
+  }
+  have.store(count + 1, std::memory_order_relaxed);
+  return count;
+}
+
 int attn(const dsa_kv_attn_args_t* a, void* stream) {
   if (!a) return DSA_KV_ERR_NULL_POINTER;
   if (a->struct_size != sizeof(*a)) return DSA_KV_ERR_BAD_ARGS_SIZE;
@@ -109,19 +135,39 @@ int attn(const dsa_kv_attn_args_t* a, void* stream) {
       return DSA_KV_ERR_CUDA;
     granted.store(true, std::memory_order_relaxed);
   }
-  // Few tiles: as many CTAs to each as stay resident at once, as long as every
-  // warp has a chunk. Measured (us with 1 / 2 / 4 / 8 CTAs per tile; two fitted an
-  // SM): 8 tiles of 32 chunks 15.6 / 11.3 / 9.4 / 8.9, 128 tiles of 64 chunks
-  // 34.4 / 27.2 / 32 / 43, 256 tiles of 128 chunks 91.5 / 96.3 / 105 / 136.
-  const int64_t resident = (int64_t)sms * v.ctas;
-  int cluster = 1;
-  while (cluster < kMaxCluster && tiles * cluster * 2 <= resident && items >= (int64_t)cluster * 2 * kAttnWarps) cluster *= 2;
+  // CTAs to a tile: what ends first. Of the tile's rounds (a chunk to each warp)
+  // a cluster takes its share; joining 2, 4 or 8 CTAs takes as long as 1.5, 2 or
+  // 2.5 rounds, and n CTAs on an SM make a round (n + 1) / 2 as long. A cluster is
+  // taken only where all tiles' are resident at once. Measured (us with 1 / 2 / 4 /
+  // 8 CTAs, 4 query heads, D = 128): 8 tiles of 8 chunks 6.3 / 6.8 / 7.3 / 7.3, of
+  // 16 chunks 9.2 / 8.3 / 7.3 / 7.5, of 32 chunks 14.9 / 11.2 / 8.7 / 7.7; 64 tiles
+  // of 32 chunks 16.0 / 12.4 / 11.4 / 18.5; 144 tiles of 16 chunks 12.2 / 13.0 /
+  // 19.4 / 30.9. Over 738 cases of every head size the choice is 1.6 % off the best
+  // in the mean and 24 % at worst; as many CTAs as the SMs hold were 5.6 %, and up
+  // to 82 % where clusters did not fit the groups of SMs that hold one together.
+  int log_c = 0, per_sm = tiles <= (int64_t)sms * v.ctas ? (int)ceil_div(tiles, sms) : v.ctas;
+  {
+    const int join2[4] = {0, 3, 4, 5};  // twice the rounds of a join
+    int64_t best = ceil_div(items, kAttnWarps) * (per_sm + 1);
+    for (int l = 1; (1 << l) <= kMaxCluster && items > (int64_t)(kAttnWarps << (l - 1)); ++l) {
+      int n = 1;
+      while (n <= v.ctas && max_clusters(v, dev, n, l) < tiles) ++n;
+      if (n > v.ctas) break;  // larger ones do not fit either
+      const int64_t cost = ceil_div(items, kAttnWarps << l) * (n + 1) + join2[l];
+      if (cost < best) {
+        best = cost;
+        log_c = l;
+        per_sm = n;
+      }
+    }
+  }
+  const int cluster = 1 << log_c;
 
   // A grid of at most one wave spreads evenly over the SMs only if no more CTAs
   // than its share fit one, because the next launch's are placed wherever the
   // last ones of this leave room: shared memory is asked for until that is so
   // (256 tiles of 8 heads, 8192 tokens: 87.0 instead of 96.0 us call after call).
-  const int64_t grid = tiles * cluster, per_sm = ceil_div(grid, sms);
+  const int64_t grid = tiles * cluster, resident = (int64_t)sms * v.ctas;
   const bool early = grid * 2 <= resident;
   size_t smem = v.smem + (cluster - 1) * v.more;
   if (!early && per_sm < v.ctas) {

@@ -146,7 +146,9 @@ inline CUfunction kernel_handle(const void* fn, int dev) {
 
 // Launch on the current device, in clusters of `cluster` CTAs, with
 // programmatic stream serialisation: the kernel waits for the previous one
-// (griddepcontrol.wait) before its first global access.
+// (griddepcontrol.wait) before its first global access. Without it a rotation
+// of one token took 4.1 instead of 3.4 us call after call, a write followed by a
+// read 10.6 instead of 7.7 us.
 template <typename... A>
 int launch(void (*fn)(A...), int64_t grid, int threads, size_t smem, int cluster, void* stream, const A&... args) {
   if (grid > kMaxIndex) return DSA_KV_ERR_UNSUPPORTED;

@@ -131,6 +131,14 @@ def test_selection_sizes(dev, K, NB):
     case(dev, 2, 1, 1, 8, 128, 64, min(K, 40), min(NB, 60), FP16, E4M3, seed=K + 1)
 
 
+@pytest.mark.parametrize("D,G", [(64, 4), (64, 16), (128, 4), (128, 16), (256, 4), (256, 16)])
+def test_rows_shared_by_clusters(dev, D, G):
+    """Numbers of rows and of blocks where the share of one, two, four and eight CTAs changes: too many rows for
+    clusters to be resident, one chunk to a warp and less, uneven last rounds."""
+    for B, K in ((1, 9), (1, 12), (1, 33), (37, 13), (37, 24), (76, 9), (149, 13)):
+        case(dev, B, 1, 1, G, D, 64, K, K + 1, BF16, E4M3, seed=B + K)
+
+
 @pytest.mark.parametrize("how", ["nhd", "pair"])
 def test_cache_layouts(dev, how):
     case(dev, 2, 1, 3, 4, 128, 48, 4, 6, BF16, E4M3, seed=3, how=how)
