@@ -207,10 +207,8 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
                : "memory");
   return v;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 
 // Place of float4 `f4` of head `row` in a warp's partial result: the units of a
 // head are permuted so that the lanes' writes spread over the banks.
@@ -723,10 +721,12 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
         part[row * D + ((16 * y + 8 + g) ^ (c << 3))] = o[y][x][2 + e];
       }
     }
-  if (C > 1)
-    cluster_sync();
-  else
+  if (C > 1) {
+    cluster_arrive();
+    cluster_wait();
+  } else {
     __syncthreads();
+  }
 
   // Join. Every CTA of the cluster works out the weights of all NW warps, a
   // group of lanes per head, and then its share of the output, as many lanes to
@@ -734,6 +734,31 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
   // took 2 us longer with 32 warps: each walked through all of them.)
   float* const all = reinterpret_cast<float*>(smem + L::all);
   float* const fin = reinterpret_cast<float*>(smem + L::fin);
+  const int units = rows * (D / 4);
+  // In a cluster: four values of the output go to 2^log_lanes lanes. Where a lane
+  // has few partial results, they are on their way while the weights are worked
+  // out (one row of 4 heads over 2048 tokens, D = 128: 7.0 instead of 7.6 us).
+  constexpr int AHEAD = 8;
+  int share = 0, log_lanes = 0;
+  uint32_t first_n = 0;
+  bool few = false;
+  float4 ahead[AHEAD];
+  if (C > 1) {
+    share = (units + (int)C - 1) >> (__ffs(C) - 1);
+    while (log_lanes < 4 && (2u << log_lanes) <= NW && (share << (log_lanes + 1)) <= kAttnThreads) ++log_lanes;
+    first_n = threadIdx.x & ((1u << log_lanes) - 1);
+    few = log_lanes > 0 && (NW >> log_lanes) <= AHEAD;
+    if (few) {
+      const int at = (int)(threadIdx.x >> log_lanes), i = rank * share + at;
+      const bool mine = at < share && i < units;
+      const uint32_t off = base + (uint32_t)L::ring + (mine ? part_index<D>(i / (D / 4), i % (D / 4)) * 16 : 0);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const uint32_t n = first_n + ((uint32_t)k << log_lanes);
+        if (n < NW) ahead[k] = ld_cluster4(mapa(off + (n % W) * (uint32_t)L::region, n / W));
+      }
+    }
+  }
   {
     constexpr int LPR = kAttnThreads / R;  // lanes of a head: 16 or 8
     constexpr int MOST = kMaxCluster * W / LPR;
@@ -785,7 +810,6 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     v.y = Half16<T>::pack(acc.z * f, acc.w * f);
     *reinterpret_cast<uint2*>(p.out.row(b, qi, head0 + row) + f4 * 8) = v;
   };
-  const int units = rows * (D / 4);
   if (C == 1) {
 #pragma unroll 4
     for (int i = threadIdx.x; i < units; i += kAttnThreads) {
@@ -804,33 +828,41 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     }
     return;
   }
-  const int share = (units + (int)C - 1) / (int)C;
-  int log_lanes = 0;
-  while (log_lanes < 4 && (2u << log_lanes) <= NW && (share << (log_lanes + 1)) <= kAttnThreads) ++log_lanes;
   for (int i0 = 0; i0 < share; i0 += kAttnThreads >> log_lanes) {
-    const int i = rank * share + i0 + (threadIdx.x >> log_lanes);
-    const bool mine = i0 + (int)(threadIdx.x >> log_lanes) < share && i < units;
+    const int at = i0 + (int)(threadIdx.x >> log_lanes), i = rank * share + at;
+    const bool mine = at < share && i < units;
     const int row = mine ? i / (D / 4) : 0, f4 = mine ? i % (D / 4) : 0;
     const uint32_t off = base + (uint32_t)L::ring + part_index<D>(row, f4) * 16;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (uint32_t n = threadIdx.x & ((1u << log_lanes) - 1); n < NW; n += 1u << log_lanes) {
-      const float4 v = ld_cluster4(mapa(off + (n % W) * (uint32_t)L::region, n / W));
+    auto add = [&](uint32_t n, const float4& v) {
       const float w = all[n * R + row];
       acc.x = fmaf(w, v.x, acc.x);
       acc.y = fmaf(w, v.y, acc.y);
       acc.z = fmaf(w, v.z, acc.z);
       acc.w = fmaf(w, v.w, acc.w);
+    };
+    if (few) {
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const uint32_t n = first_n + ((uint32_t)k << log_lanes);
+        if (n < NW) add(n, ahead[k]);
+      }
+    } else {
+#pragma unroll 4
+      for (uint32_t n = first_n; n < NW; n += 1u << log_lanes)
+        add(n, ld_cluster4(mapa(off + (n % W) * (uint32_t)L::region, n / W)));
     }
+    // shared memory stays until every CTA has read it
+    if (i0 + (kAttnThreads >> log_lanes) >= share) cluster_arrive();
     for (int y = 1; y < 1 << log_lanes; y <<= 1) {
       acc.x += __shfl_xor_sync(0xffffffffu, acc.x, y);
       acc.y += __shfl_xor_sync(0xffffffffu, acc.y, y);
       acc.z += __shfl_xor_sync(0xffffffffu, acc.z, y);
       acc.w += __shfl_xor_sync(0xffffffffu, acc.w, y);
     }
-    if (mine && (threadIdx.x & ((1u << log_lanes) - 1)) == 0) store(row, f4, acc);
+    if (mine && first_n == 0) store(row, f4, acc);
   }
-  cluster_sync();  // shared memory stays until every CTA has read it
+  cluster_wait();
 }
 
 }  // namespace kv
