@@ -721,46 +721,85 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
         part[row * D + ((16 * y + 8 + g) ^ (c << 3))] = o[y][x][2 + e];
       }
     }
-  if (C > 1) {
-    cluster_arrive();
-    cluster_wait();
-  } else {
+  // Join. out = sum_n w_n o_n / sum_n w_n l_n over the warps, w_n = 2^(M_n - max).
+  constexpr int LPR = kAttnThreads / R;  // lanes of a head: 16 or 8
+  auto finish = [&](float total) { return total == 0.f ? 0.f : 1.0f / total; };
+  auto put_lse = [&](int row, float m, float total) {
+    p.lse[((int64_t)b * p.Q.d + qi) * p.H.d * p.G + head0 + row] =
+        total == 0.f ? -INFINITY : (m - kLift + log2f(total)) * 0.69314718055994531f;
+  };
+  auto store = [&](int row, int f4, const float4& acc, float f) {
+    uint2 v;
+    v.x = Half16<T>::pack(acc.x * f, acc.y * f);
+    v.y = Half16<T>::pack(acc.z * f, acc.w * f);
+    *reinterpret_cast<uint2*>(p.out.row(b, qi, head0 + row) + f4 * 8) = v;
+  };
+  if (C == 1) {
+    // Every thread works the weights of its head out for itself: 0.4 us less than
+    // weights by groups of lanes and a barrier.
     __syncthreads();
+    const int row = threadIdx.x / LPR, sub = threadIdx.x % LPR;
+    if (row >= rows) return;
+    float w[W], m = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int n = 0; n < W; ++n) {
+      w[n] = ml[n * 2 * R + row];
+      m = fmaxf(m, w[n]);
+    }
+    const float from_all = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int n = 0; n < W; ++n) {
+      w[n] = exp2_approx(w[n] - from_all);
+      total = fmaf(w[n], ml[n * 2 * R + R + row], total);
+    }
+    const float f = finish(total);
+#pragma unroll
+    for (int k = 0; k < D / 4 / LPR; ++k) {
+      const int f4 = sub + k * LPR, at = part_index<D>(row, f4);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int n = 0; n < W; ++n) {
+        const float4 v = reinterpret_cast<const float4*>(smem + L::ring + n * L::region)[at];
+        acc.x = fmaf(w[n], v.x, acc.x);
+        acc.y = fmaf(w[n], v.y, acc.y);
+        acc.z = fmaf(w[n], v.z, acc.z);
+        acc.w = fmaf(w[n], v.w, acc.w);
+      }
+      store(row, f4, acc, f);
+    }
+    if (sub == 0 && p.lse) put_lse(row, m, total);
+    return;
   }
 
-  // Join. Every CTA of the cluster works out the weights of all NW warps, a
-  // group of lanes per head, and then its share of the output, as many lanes to
-  // four values as there are to spare. (A thread per head and per four values
-  // took 2 us longer with 32 warps: each walked through all of them.)
+  // Every CTA of the cluster works out the weights of all NW warps, a group of
+  // lanes per head, and then its share of the output, as many lanes to four values
+  // as there are to spare. (A thread per head and per four values took 2 us longer
+  // with 32 warps: each walked through all of them.)
+  cluster_arrive();
+  cluster_wait();
   float* const all = reinterpret_cast<float*>(smem + L::all);
   float* const fin = reinterpret_cast<float*>(smem + L::fin);
-  const int units = rows * (D / 4);
-  // In a cluster: four values of the output go to 2^log_lanes lanes. Where a lane
-  // has few partial results, they are on their way while the weights are worked
-  // out (one row of 4 heads over 2048 tokens, D = 128: 7.0 instead of 7.6 us).
+  // Four values go to 2^log_lanes lanes. Where a lane has few partial results,
+  // they are on their way while the weights are worked out (one row of 4 heads
+  // over 2048 tokens, D = 128: 7.0 instead of 7.6 us).
   constexpr int AHEAD = 8;
-  int share = 0, log_lanes = 0;
-  uint32_t first_n = 0;
-  bool few = false;
+  const int units = rows * (D / 4), share = (units + (int)C - 1) >> (__ffs(C) - 1);
+  int log_lanes = 0;
+  while (log_lanes < 4 && (2u << log_lanes) <= NW && (share << (log_lanes + 1)) <= kAttnThreads) ++log_lanes;
+  const uint32_t first_n = threadIdx.x & ((1u << log_lanes) - 1);
+  const bool few = log_lanes > 0 && (NW >> log_lanes) <= AHEAD;
   float4 ahead[AHEAD];
-  if (C > 1) {
-    share = (units + (int)C - 1) >> (__ffs(C) - 1);
-    while (log_lanes < 4 && (2u << log_lanes) <= NW && (share << (log_lanes + 1)) <= kAttnThreads) ++log_lanes;
-    first_n = threadIdx.x & ((1u << log_lanes) - 1);
-    few = log_lanes > 0 && (NW >> log_lanes) <= AHEAD;
-    if (few) {
-      const int at = (int)(threadIdx.x >> log_lanes), i = rank * share + at;
-      const bool mine = at < share && i < units;
-      const uint32_t off = base + (uint32_t)L::ring + (mine ? part_index<D>(i / (D / 4), i % (D / 4)) * 16 : 0);
+  if (few) {
+    const int at = (int)(threadIdx.x >> log_lanes), i = rank * share + at;
+    const bool mine = at < share && i < units;
+    const uint32_t off = base + (uint32_t)L::ring + (mine ? part_index<D>(i / (D / 4), i % (D / 4)) * 16 : 0);
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const uint32_t n = first_n + ((uint32_t)k << log_lanes);
-        if (n < NW) ahead[k] = ld_cluster4(mapa(off + (n % W) * (uint32_t)L::region, n / W));
-      }
+    for (int k = 0; k < AHEAD; ++k) {
+      const uint32_t n = first_n + ((uint32_t)k << log_lanes);
+      if (n < NW) ahead[k] = ld_cluster4(mapa(off + (n % W) * (uint32_t)L::region, n / W));
     }
   }
   {
-    constexpr int LPR = kAttnThreads / R;  // lanes of a head: 16 or 8
     constexpr int MOST = kMaxCluster * W / LPR;
     const int row = threadIdx.x / LPR;
     const uint32_t sub = threadIdx.x % LPR;
@@ -770,12 +809,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
       const uint32_t n = sub + i * LPR;
       top[i] = -INFINITY;
       sum[i] = 0.f;
-      if (C == 1) {
-        if (n < W) {
-          top[i] = ml[n * 2 * R + row];
-          sum[i] = ml[n * 2 * R + R + row];
-        }
-      } else if (n < NW) {
+      if (n < NW) {
         const uint32_t at = mapa(base + (uint32_t)L::ml + ((n % W) * 2 * R + row) * 4, n / W);
         top[i] = ld_cluster(at);
         sum[i] = ld_cluster(at + R * 4);
@@ -796,38 +830,11 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
 #pragma unroll
     for (int y = 1; y < LPR; y <<= 1) total += __shfl_xor_sync(0xffffffffu, total, y);
     if (sub == 0) {
-      fin[row] = total == 0.f ? 0.f : 1.0f / total;
-      if (p.lse && rank == 0 && row < rows)
-        p.lse[((int64_t)b * p.Q.d + qi) * p.H.d * p.G + head0 + row] =
-            total == 0.f ? -INFINITY : (m - kLift + log2f(total)) * 0.69314718055994531f;
+      fin[row] = finish(total);
+      if (p.lse && rank == 0 && row < rows) put_lse(row, m, total);
     }
   }
   __syncthreads();
-  auto store = [&](int row, int f4, const float4& acc) {
-    const float f = fin[row];
-    uint2 v;
-    v.x = Half16<T>::pack(acc.x * f, acc.y * f);
-    v.y = Half16<T>::pack(acc.z * f, acc.w * f);
-    *reinterpret_cast<uint2*>(p.out.row(b, qi, head0 + row) + f4 * 8) = v;
-  };
-  if (C == 1) {
-#pragma unroll 4
-    for (int i = threadIdx.x; i < units; i += kAttnThreads) {
-      const int row = i / (D / 4), f4 = i % (D / 4), at = part_index<D>(row, f4);
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int n = 0; n < W; ++n) {
-        const float4 v = reinterpret_cast<const float4*>(smem + L::ring + n * L::region)[at];
-        const float w = all[n * R + row];
-        acc.x = fmaf(w, v.x, acc.x);
-        acc.y = fmaf(w, v.y, acc.y);
-        acc.z = fmaf(w, v.z, acc.z);
-        acc.w = fmaf(w, v.w, acc.w);
-      }
-      store(row, f4, acc);
-    }
-    return;
-  }
   for (int i0 = 0; i0 < share; i0 += kAttnThreads >> log_lanes) {
     const int at = i0 + (int)(threadIdx.x >> log_lanes), i = rank * share + at;
     const bool mine = at < share && i < units;
@@ -860,7 +867,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
       acc.z += __shfl_xor_sync(0xffffffffu, acc.z, y);
       acc.w += __shfl_xor_sync(0xffffffffu, acc.w, y);
     }
-    if (mine && first_n == 0) store(row, f4, acc);
+    if (mine && first_n == 0) store(row, f4, acc, fin[row]);
   }
   cluster_wait();
 }
