@@ -24,10 +24,13 @@ CacheSide side(void* codes, float* scale, const int64_t s[3], const int64_t ss[3
 int lanes_of(int64_t D) { return D <= 64 ? 8 : D <= 128 ? 16 : 32; }
 
 using RopeFn = void (*)(const RopeParams);
+template <typename T, bool I, int U>
+RopeFn rope_fn_u(int lanes) {
+  return lanes == 8 ? rope_kernel<T, 8, U, I> : lanes == 16 ? rope_kernel<T, 16, U, I> : rope_kernel<T, 32, U, I>;
+}
 template <typename T, bool I>
-RopeFn rope_fn(int lanes) {
-  return lanes == 8 ? rope_kernel<T, 8, kRopeUnroll, I>
-                    : lanes == 16 ? rope_kernel<T, 16, kRopeUnroll, I> : rope_kernel<T, 32, kRopeUnroll, I>;
+RopeFn rope_fn(int lanes, int u) {
+  return u == 2 ? rope_fn_u<T, I, 2>(lanes) : rope_fn_u<T, I, 4>(lanes);
 }
 
 using CopyFn = void (*)(const CopyParams);
@@ -72,8 +75,21 @@ int rope(const dsa_kv_rope_args_t* a, void* stream) {
       !aligned(a->positions, ib))
     return DSA_KV_ERR_ALIGNMENT;
 
-  const int lanes = lanes_of(a->D), heads = 32 / lanes * kRopeUnroll;  // of a step
-  const int64_t steps_q = ceil_div(a->Hq, heads), per_token = steps_q + ceil_div(a->Hk, heads);
+  int dev, sms;
+  if (!bind_device(&dev) || !sm_count(dev, &sms)) return DSA_KV_ERR_CUDA;
+  // Steps of two heads to a group of lanes where each then has a warp to itself on
+  // one CTA per SM, else of four. Device time in us with two / four, 40 heads x
+  // 128: 1 token 2.16 / 2.47, 32 tokens 2.37 / 2.77, 96 tokens 2.46 / 2.87, 128
+  // tokens (160 CTAs) 2.98 / 2.88, 384 tokens 3.90 / 3.49, 8192 tokens 49 / 33.4.
+  const int lanes = lanes_of(a->D);
+  int u = 2;
+  int64_t steps_q, per_token;
+  for (;; u = 4) {
+    const int heads = 32 / lanes * u;  // of a step
+    steps_q = ceil_div(a->Hq, heads);
+    per_token = steps_q + ceil_div(a->Hk, heads);
+    if (u == 4 || a->B * a->Q * per_token <= (int64_t)sms * kRopeWarps) break;
+  }
   RopeParams p;
   p.q = dense(a->q);
   p.k = dense(a->k);
@@ -98,11 +114,9 @@ int rope(const dsa_kv_rope_args_t* a, void* stream) {
   p.eps = a->eps;
   p.inv_d = 1.0f / (float)a->D;
   const RopeFn fn = a->dtype == DSA_KV_BF16
-                        ? (a->interleaved ? rope_fn<__nv_bfloat16, true>(lanes) : rope_fn<__nv_bfloat16, false>(lanes))
-                        : (a->interleaved ? rope_fn<__half, true>(lanes) : rope_fn<__half, false>(lanes));
+                        ? (a->interleaved ? rope_fn<__nv_bfloat16, true>(lanes, u) : rope_fn<__nv_bfloat16, false>(lanes, u))
+                        : (a->interleaved ? rope_fn<__half, true>(lanes, u) : rope_fn<__half, false>(lanes, u));
   // A warp for every step, as far as they are all resident at once.
-  int dev, sms;
-  if (!bind_device(&dev) || !sm_count(dev, &sms)) return DSA_KV_ERR_CUDA;
   const int64_t most = (int64_t)sms * kRopeCtas, grid = ceil_div(p.steps, kRopeWarps);
   return launch(fn, grid < most ? grid : most, kRopeThreads, 0, 1, stream, p);
 }

@@ -25,7 +25,6 @@
 
 namespace kv {
 
-constexpr int kRopeUnroll = 4;  // heads that a group of lanes holds at a time
 constexpr int kRopeThreads = 256, kRopeWarps = kRopeThreads / 32;
 constexpr int kRopeCtas = 2;    // CTAs per SM
 

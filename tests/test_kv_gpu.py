@@ -102,6 +102,24 @@ def test_rope_padding_far_positions_and_in_place(dev, inter):
     check_rope(dev, q, k, gq, gk, angles(300, 64), pos, interleaved=inter, in_place=True)
 
 
+@pytest.mark.parametrize("B,Q,Hq,Hk,D,rot,dtype,gdt,inter", [
+    (3, 700, 5, 1, 128, 128, BF16, BF16, False),
+    (2, 1201, 9, 2, 64, 32, FP16, FP32, True),
+    (1, 1500, 3, 3, 256, 256, BF16, FP32, False),
+    (2, 611, 18, 0, 96, 64, FP16, FP16, False),
+    (1, 1185, 2, 2, 192, 128, BF16, FP32, True),
+    (37, 32, 1, 0, 128, 128, BF16, BF16, False),
+], ids=str)
+def test_rope_many_tokens(dev, B, Q, Hq, Hk, D, rot, dtype, gdt, inter):
+    """More steps than warps: each walks over several, through padded tokens, ends of sequences and far positions."""
+    q, k, gq, gk, pos = rope_inputs(B, Q, Hq, Hk, D, dtype, gdt, seed=B + Q)
+    g = gen(Q)
+    pos = torch.where(torch.rand(pos.shape, generator=g) < 0.1, -1, pos)
+    pos[:, -3:] = -1
+    pos[0, 5], pos[-1, 9] = 300, 2 ** 30
+    check_rope(dev, q, k, gq, gk, angles(300, rot), pos, interleaved=inter)
+
+
 def test_rope_zero_and_huge_heads(dev):
     q, k, gq, gk, pos = rope_inputs(1, 4, 2, 2, 128, BF16, FP32, seed=6)
     q = q.clone()
