@@ -49,9 +49,9 @@
 // have to be written back to shared memory as fp16 first.
 //
 // What bounds it: a decode batch is bound by HBM (32 rows x 8 key heads over 8192
-// e4m3 tokens of D = 128: 88 us, 6.3 TB/s). Rows whose pages stay in L2 are bound
+// e4m3 tokens of D = 128: 87 us, 6.4 TB/s). Rows whose pages stay in L2 are bound
 // by what the warps issue: 265 cycles per SM for 32 tokens of 16 heads at
-// D = 128 (1024 rows x 2048 tokens: 88 us), of which the tensor pipe needs 128
+// D = 128 (1024 rows x 2048 tokens: 85.5 us), of which the tensor pipe needs 128
 // and the conversion of codes, on the half-rate integer pipe, 64.
 #pragma once
 
