@@ -120,6 +120,12 @@ def test_block_sizes(dev, bs):
     case(dev, 1, 2, 1, 2, 64, bs, 40, 50, FP16, INT8, seed=bs + 1)
 
 
+@pytest.mark.parametrize("bs", [200, 1000, 4096])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_long_blocks(dev, bs, D):
+    case(dev, 2, 3, 1, 4, D, bs, 2, 3, BF16, E4M3, seed=bs + D)
+
+
 @pytest.mark.parametrize("G", [1, 2, 7, 8, 9, 15, 16, 17, 32, 40])
 def test_query_heads_per_key_head(dev, G):
     case(dev, 1, 2, 2, G, 128, 32, 4, 6, BF16, E4M3, seed=G)
@@ -545,3 +551,51 @@ def test_a_first_call_from_a_thread_without_a_context(dev):
 def test_a_long_row(dev):
     """One row over 8192 selected tokens of a large cache: the sums of the oracle, the bound on n/16 steps."""
     case(dev, 1, 1, 1, 8, 128, 64, 128, 140, BF16, E4M3, seed=50, full=True)
+
+
+@pytest.mark.parametrize("code", [E4M3, INT8])
+def test_offsets_beyond_32_bits(dev, code):
+    """A cache of 9 GB, keys and values side by side, against a compact one of the pages in use; queries, new tokens
+    and outputs with more than 4 GiB between their sequences. Same bits; the pages 2^32 bytes below stay as they were."""
+    B, Q, Hq, H, D, bs, NB, K = 2, 256, 8, 8, 128, 64, 4, 3
+    P, below = 70000, 2 ** 32 // (2 * H * bs * D)  # pages of 128 KiB
+    g = gen(51)
+    high = torch.tensor([[69999, 32768, 50000, 40001], [33000, 65535, 65000, 69000]])
+    codes = torch.empty(P, 2, H, bs, D, dtype=torch.uint8, device=dev)
+    scales = torch.empty(P, 2, H, bs, device=dev)
+    codes[(high - below).to(dev)] = 17
+    scales[(high - below).to(dev)] = 17.0
+    big = (codes[:, 0].view(code), scales[:, 0], codes[:, 1].view(code), scales[:, 1])
+    small = tuple(torch.zeros(B * NB, *t.shape[1:], dtype=t.dtype if t.dtype != code else torch.uint8, device=dev)
+                  for t in big)
+    small = tuple(t.view(code) if t.dtype == torch.uint8 else t for t in small)
+    far = 2 ** 31 + 2 ** 20  # elements from one sequence to the next
+    buf = torch.empty(far + 4 * Q * Hq * D, dtype=BF16, device=dev)
+
+    def apart(n, t):  # the n-th tensor of such a buffer
+        v = buf[n * Q * Hq * D:].as_strided((B, Q, Hq, D), (far, Hq * D, D, 1))
+        return v if t is None else v.copy_(t)
+
+    q, k, v = (torch.randn(B, Q, Hq, D, generator=g).to(BF16).to(dev) for _ in range(3))
+    gamma, cs = torch.ones(D, device=dev), angles(NB * bs, D).to(dev)
+    pos = torch.arange(Q).expand(B, Q).contiguous().int().to(dev)
+    lens = torch.tensor([Q, Q - 5], dtype=torch.int32, device=dev)
+    blocks = torch.rand(B, H, Q, NB, generator=g).argsort(-1)[..., :K].contiguous()
+    got = []
+    for cache, table, wide in ((big, high, True), (small, torch.arange(B * NB).view(B, NB), False)):
+        pages = table[:, None, None].expand(B, H, Q, NB).gather(3, blocks).to(dev)
+        a, b, c = (apart(n, t) if wide else t.clone() for n, t in enumerate((q, k, v)))
+        out = apart(3, None) if wide else torch.empty_like(a)
+        lse = torch.empty(B, Q, Hq, device=dev)
+        kr, vr = (torch.zeros(B, NB * bs, H, D, dtype=BF16, device=dev) for _ in range(2))
+        td = table.to(dev)
+        qk_rmsnorm_rope(a, b, gamma, gamma, cs, pos, a, b, 1e-6)
+        paged_kv_quant_write(b, c, *cache, td, pos)
+        dsa_paged_attention(a, *cache, blocks.to(dev), pages, pos, lens, out, lse, D ** -0.5)
+        paged_kv_dequant_read(*cache, td, lens, kr, vr)
+        torch.cuda.synchronize(dev)
+        got.append([t.cpu().clone() for t in (a, b, out, lse, kr, vr)])
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+    assert got[0][2].abs().max() > 0 and not any(x.isnan().any() for x in got[0])
+    assert (codes[(high - below).to(dev)] == 17).all() and (scales[(high - below).to(dev)] == 17.0).all()
