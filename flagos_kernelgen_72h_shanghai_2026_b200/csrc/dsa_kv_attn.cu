@@ -44,12 +44,12 @@ Variant variant() {
   return Variant{attn_kernel<T, D, E, NB, TOK, CTAS>, L::total(1), L::total(2) - L::total(1), TOK, CTAS};
 }
 // Tokens of a chunk, and CTAs per SM that registers are laid out for. Measured
-// (us): chunks of 64 tokens against 32 with 16 heads at D = 128, 1024 rows x
-// 2048 tokens: 95.7 against 108.5 (three CTAs of 32) and 118 (two): what a chunk
-// costs besides its products weighs more than the warps that hide it. Three
-// CTAs against two there: 102 against 88.0; with 8 heads, 2048 rows: 116
-// against 134; at D = 64, 2048 rows: 74 (four) against 81 (three) with 8 heads,
-// 104 (three) against 122 (two) with 16.
+// (us, 2048 tokens to a row): chunks of 64 tokens against 32 with 16 heads at
+// D = 128, 1024 rows: 83.0 against 85.0 (three CTAs of 32) and 100 (two): what a
+// chunk costs besides its products weighs as much as the warps that hide it. CTAs
+// with chunks of 64: three against two there 99.4 to 83.0 (spills); with 8 heads,
+// 2048 rows, 107 to 122; at D = 64 with 8 heads three / four / five 73.6 / 67.0 /
+// 68.4, with 16 heads two / three / four 112 / 94.8 / 98.1.
 template <typename T, bool E>
 Variant variant_of(int64_t D, int nb) {
   if (D == 64) return nb == 1 ? variant<T, E, 64, 1, 64, 4>() : variant<T, E, 64, 2, 64, 3>();
