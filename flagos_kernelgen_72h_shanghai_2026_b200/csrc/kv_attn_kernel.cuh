@@ -17,6 +17,12 @@
 // with M the running maximum of a_t. The value scale sits in the exponent, so
 // the weight of a token is at most 1 whatever the scales are, the products
 // run on raw codes (exact in fp16), and the maximum bounds each term of o.
+// It does not bound those of l, nor keep them near 1: where value scales differ
+// by more than 2^126, 2^(a_t - M) may be zero in fp32 and 2^(a_t - M) / vs_t not. A
+// warp that has met a scale above 2^32 (the least is 1e-12) takes the terms of l as
+// 2^(a_t - M - log2(vs_t)) from then on, times 2^24 (a row's l lies between 2^-122
+// and 2^85: a term 2^-28 of the least one still counts), and l is multiplied by
+// powers of two that may themselves be too small in two steps, here and in the join.
 //
 // Precision: q is brought to fp16 by one power of two for all heads of a CTA, the
 // largest value in [2^14, 2^15): bf16 values lose bits only 2^-28 below it.
@@ -56,6 +62,7 @@
 #pragma once
 
 #include <cuda.h>
+#include <type_traits>
 
 #include "farq_kernel.cuh"
 #include "kv_common.cuh"
@@ -67,6 +74,10 @@ constexpr int kAttnThreads = 32 * kAttnWarps;
 constexpr int kMaxCluster = 8;
 constexpr float kLift = 6.0f;      // weights are 2^(a - M + kLift)
 constexpr float kLag = 8.0f;       // M is moved when a maximum exceeds it by more
+constexpr float kWide = 4294967296.0f;  // value scales up to it: 1 / vs brings every term of l that counts back
+constexpr float kSumLift = 24.0f;       // l is 2^kSumLift times its value from there on, and in the join
+constexpr float kSumUp = 16777216.0f;   // 2^kSumLift
+constexpr float kTwoSteps = -64.0f;     // powers of two below it are applied to l in two steps
 constexpr uint64_t kAttnWaitNs = 2000000000ull;
 
 struct AttnParams {
@@ -383,15 +394,18 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
   };
   float qs = 0.f;  // softmax_scale * log2(e) over the factor of the queries
   // Factors of this lane's tokens: of their scores, the exponent and the
-  // inverse of their value scales.
+  // inverse of their value scales. True if one of them has a scale above kWide.
   auto factors = [&] {
+    bool above = false;
 #pragma unroll
     for (int t = 0; t < LT; ++t) {
       const float ks = scales[32 * t + lane];
       float vs = scales[TOK + 32 * t + lane];
       vs = vs < kMinScale ? kMinScale : vs;
+      above |= vs > kWide;
       tok[32 * t + lane] = make_float4(ks * qs, __log2f(vs), rcp_approx(vs), 0.f);
     }
+    return above;
   };
   // Rows that hold no token of the row: whatever lies there becomes zeros.
   auto clear = [&](uint8_t* box, const uint32_t (&mask)[LT]) {
@@ -532,162 +546,185 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
                          (((lane >> 4) ^ (D == 64 ? (vr >> 1) & 3 : vr & 7)) << 4);
   uint8_t* const kbox = ring;
   uint8_t* const vbox = ring + L::box;
-  for (uint32_t parity = 0; have; parity ^= 1) {
-    // this chunk's factors, the next chunk's addresses
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    factors();
-    if (more) prepare();
-    // a wait that runs out ends the loop before the next copy
-    failed = !farq::mbar_wait_bounded(bars, parity, kAttnWaitNs);
-    clear(kbox, mask);
+  uint32_t parity = 0;
+  // Works on chunks until none is left, or, where it is not `wide`, one holds a
+  // value scale above kWide: then true, and the wide copy begins with that chunk
+  // anew, its keys still in their box and the next chunk's addresses at hand. One
+  // loop with both forms of the sums was 4 % slower (1024 rows x 16 heads x 2048 tokens).
+  auto work = [&](auto is_wide) -> bool {
+    constexpr bool WIDE = decltype(is_wide)::value;
+    for (bool again = WIDE; have; parity ^= 1) {
+      // this chunk's factors, the next chunk's addresses
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      const bool above = factors();
+      if (more && !again) prepare();
+      again = false;
+      // a wait that runs out ends the loop before the next copy
+      failed = !farq::mbar_wait_bounded(bars, parity, kAttnWaitNs);
+      clear(kbox, mask);
 
-    // scores of tiles of 16 tokens
-    float sc[NS][NB][4];
-#pragma unroll
-    for (int hh = 0; hh < NH; ++hh)
-#pragma unroll
-      for (int u = 0; u < NU; ++u) {
-        uint4 kw[2 * NS];  // key rows, two of each tile
-#pragma unroll
-        for (int j = 0; j < 2 * NS; ++j) {
-          const int row = 16 * (j >> 1) + 2 * (j & 1) + g0;
-          const uint32_t at = D == 64 ? row * 64 + ((c ^ ((row >> 1) & 3)) << 4)
-                                      : hh * TOK * 128 + row * 128 + (((2 * c + u) ^ (row & 7)) << 4);
-          kw[j] = *reinterpret_cast<const uint4*>(kbox + at);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int ks = (hh * NU + u) * 4 + i;
-          uint32_t bq[NB][2];
-#pragma unroll
-          for (int x = 0; x < NB; ++x) {
-            if (QSMEM) {
-              const uint2 v = *reinterpret_cast<const uint2*>(smem + L::qf + ((ks * NB + x) * 32 + lane) * 8);
-              bq[x][0] = v.x;
-              bq[x][1] = v.y;
-            } else {
-              bq[x][0] = qf[QSMEM ? 0 : ks][x][0];
-              bq[x][1] = qf[QSMEM ? 0 : ks][x][1];
-            }
-          }
-#pragma unroll
-          for (int t = 0; t < NS; ++t) {
-            const uint4 &lo = kw[2 * t], &hi = kw[2 * t + 1];
-            uint32_t a[4];
-            decode_pairs<E4M3>(i == 0 ? lo.x : i == 1 ? lo.y : i == 2 ? lo.z : lo.w, a[0], a[2]);
-            decode_pairs<E4M3>(i == 0 ? hi.x : i == 1 ? hi.y : i == 2 ? hi.z : hi.w, a[1], a[3]);
-#pragma unroll
-            for (int x = 0; x < NB; ++x) {
-              if (hh + u + i == 0)
-                mma16816_first(sc[t][x], a, bq[x][0], bq[x][1]);
-              else
-                mma16816(sc[t][x], a, bq[x][0], bq[x][1]);
-            }
-          }
-        }
-      }
-    __syncwarp();  // the keys and the scales are read, the factors written
-    if (__any_sync(0xffffffffu, failed)) break;
-    if (more) {
-      copy(&k_map, 0);
-      copy_scales();
-    }
-
-    // exponents of heads 2c, 2c + 1. M moves when a lane sees a value well above
-    // it; until then nothing has to be exchanged between lanes.
-    f32x2 a[2 * NS][NB];
-    float inv[2 * NS], m[NB][2];
-    bool partial = false;
-#pragma unroll
-    for (int t = 0; t < LT; ++t) partial |= mask[t] != 0xffffffffu;
-#pragma unroll
-    for (int j = 0; j < 2 * NS; ++j) {
-      const float4 f = tok[16 * (j >> 1) + 2 * (j & 1) + g0];
-      inv[j] = f.z;
-#pragma unroll
-      for (int x = 0; x < NB; ++x)
-        a[j][x] = fma2(pair(sc[j >> 1][x][(j & 1) * 2], sc[j >> 1][x][(j & 1) * 2 + 1]), pair(f.x, f.x), pair(f.y, f.y));
-    }
-    if (partial) {
-#pragma unroll
-      for (int j = 0; j < 2 * NS; ++j)
-#pragma unroll
-        for (int x = 0; x < NB; ++x)
-          if (!((mask[j / 4] >> (16 * ((j >> 1) & 1) + 2 * (j & 1) + g0)) & 1)) a[j][x] = pair(-INFINITY, -INFINITY);
-    }
-    bool moves = false;
-#pragma unroll
-    for (int x = 0; x < NB; ++x) {
-      m[x][0] = m[x][1] = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 2 * NS; j += 2) {
-        const float2 v = both(a[j][x]), w = both(a[j + 1][x]);
-        m[x][0] = max3(m[x][0], v.x, w.x);
-        m[x][1] = max3(m[x][1], v.y, w.y);
-      }
-      moves |= m[x][0] > M[x][0] + kLag || m[x][1] > M[x][1] + kLag;
-    }
-    if (__any_sync(0xffffffffu, moves)) {
-#pragma unroll
-      for (int x = 0; x < NB; ++x) {
-        float f[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-#pragma unroll
-          for (int y = 4; y <= 16; y <<= 1) m[x][e] = fmaxf(m[x][e], __shfl_xor_sync(0xffffffffu, m[x][e], y));
-          const float top = fmaxf(M[x][e], m[x][e]);
-          f[e] = M[x][e] == top ? 1.f : exp2_approx(M[x][e] - top);
-          M[x][e] = top;
-        }
-        l[x] = mul2(l[x], pair(f[0], f[1]));
-        from[x] = pair(kLift - (M[x][0] == -INFINITY ? 0.f : M[x][0]), kLift - (M[x][1] == -INFINITY ? 0.f : M[x][1]));
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          o[i][x][0] *= f[0];
-          o[i][x][1] *= f[1];
-          o[i][x][2] *= f[0];
-          o[i][x][3] *= f[1];
-        }
-      }
-    }
-    // weights, as the columns of the second product: rows 2c, 2c + 1 of head g
-    uint32_t pw[2 * NS][NB];
-#pragma unroll
-    for (int x = 0; x < NB; ++x)
-#pragma unroll
-      for (int j = 0; j < 2 * NS; ++j) {
-        const float2 e = both(add2(a[j][x], from[x]));
-        const float w0 = exp2_approx(e.x), w1 = exp2_approx(e.y);
-        l[x] = fma2(pair(w0, w1), pair(inv[j], inv[j]), l[x]);
-        pw[j][x] = transpose8x8(Half16<__half>::pack(w0, w1));
-      }
-
-    failed = !farq::mbar_wait_bounded(bars + 8, parity, kAttnWaitNs);
-    clear(vbox, mask);
-    // values times weights: rows g and g + 8 of output tile y are values 16y + g and 16y + g + 8
-#pragma unroll
-    for (int t = 0; t < NS; ++t)
+      // scores of tiles of 16 tokens
+      float sc[NS][NB][4];
 #pragma unroll
       for (int hh = 0; hh < NH; ++hh)
 #pragma unroll
-        for (int y = 0; y < NT / NH; y += 2) {
-          uint32_t w[4];
-          load_transposed(w, (vaddr + t * 16 * ROWB + hh * TOK * 128) ^ (y << 4));
+        for (int u = 0; u < NU; ++u) {
+          uint4 kw[2 * NS];  // key rows, two of each tile
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            uint32_t a[4];
-            decode_pairs<E4M3>(w[2 * e], a[0], a[2]);
-            decode_pairs<E4M3>(w[2 * e + 1], a[1], a[3]);
+          for (int j = 0; j < 2 * NS; ++j) {
+            const int row = 16 * (j >> 1) + 2 * (j & 1) + g0;
+            const uint32_t at = D == 64 ? row * 64 + ((c ^ ((row >> 1) & 3)) << 4)
+                                        : hh * TOK * 128 + row * 128 + (((2 * c + u) ^ (row & 7)) << 4);
+            kw[j] = *reinterpret_cast<const uint4*>(kbox + at);
+          }
 #pragma unroll
-            for (int x = 0; x < NB; ++x) mma16816(o[hh * 8 + y + e][x], a, pw[2 * t][x], pw[2 * t + 1][x]);
+          for (int i = 0; i < 4; ++i) {
+            const int ks = (hh * NU + u) * 4 + i;
+            uint32_t bq[NB][2];
+#pragma unroll
+            for (int x = 0; x < NB; ++x) {
+              if (QSMEM) {
+                const uint2 v = *reinterpret_cast<const uint2*>(smem + L::qf + ((ks * NB + x) * 32 + lane) * 8);
+                bq[x][0] = v.x;
+                bq[x][1] = v.y;
+              } else {
+                bq[x][0] = qf[QSMEM ? 0 : ks][x][0];
+                bq[x][1] = qf[QSMEM ? 0 : ks][x][1];
+              }
+            }
+#pragma unroll
+            for (int t = 0; t < NS; ++t) {
+              const uint4 &lo = kw[2 * t], &hi = kw[2 * t + 1];
+              uint32_t a[4];
+              decode_pairs<E4M3>(i == 0 ? lo.x : i == 1 ? lo.y : i == 2 ? lo.z : lo.w, a[0], a[2]);
+              decode_pairs<E4M3>(i == 0 ? hi.x : i == 1 ? hi.y : i == 2 ? hi.z : hi.w, a[1], a[3]);
+#pragma unroll
+              for (int x = 0; x < NB; ++x) {
+                if (hh + u + i == 0)
+                  mma16816_first(sc[t][x], a, bq[x][0], bq[x][1]);
+                else
+                  mma16816(sc[t][x], a, bq[x][0], bq[x][1]);
+              }
+            }
           }
         }
-    __syncwarp();  // the values and the factors are read
-    if (__any_sync(0xffffffffu, failed)) break;
-    have = more;
-    if (more) copy(&v_map, 1);
+      __syncwarp();  // the keys and the scales are read, the factors written
+      if (__any_sync(0xffffffffu, failed || (above && !WIDE))) return !__any_sync(0xffffffffu, failed);
+      if (more) {
+        copy(&k_map, 0);
+        copy_scales();
+      }
+
+      // exponents of heads 2c, 2c + 1. M moves when a lane sees a value well above
+      // it; until then nothing has to be exchanged between lanes.
+      f32x2 a[2 * NS][NB];
+      float inv[2 * NS], m[NB][2];
+      bool partial = false;
 #pragma unroll
-    for (int t = 0; t < LT; ++t) mask[t] = cp_mask[t];
+      for (int t = 0; t < LT; ++t) partial |= mask[t] != 0xffffffffu;
+#pragma unroll
+      for (int j = 0; j < 2 * NS; ++j) {
+        const float4 f = tok[16 * (j >> 1) + 2 * (j & 1) + g0];
+        inv[j] = f.z;
+#pragma unroll
+        for (int x = 0; x < NB; ++x)
+          a[j][x] = fma2(pair(sc[j >> 1][x][(j & 1) * 2], sc[j >> 1][x][(j & 1) * 2 + 1]), pair(f.x, f.x), pair(f.y, f.y));
+      }
+      if (partial) {
+#pragma unroll
+        for (int j = 0; j < 2 * NS; ++j)
+#pragma unroll
+          for (int x = 0; x < NB; ++x)
+            if (!((mask[j / 4] >> (16 * ((j >> 1) & 1) + 2 * (j & 1) + g0)) & 1)) a[j][x] = pair(-INFINITY, -INFINITY);
+      }
+      bool moves = false;
+#pragma unroll
+      for (int x = 0; x < NB; ++x) {
+        m[x][0] = m[x][1] = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 2 * NS; j += 2) {
+          const float2 v = both(a[j][x]), w = both(a[j + 1][x]);
+          m[x][0] = max3(m[x][0], v.x, w.x);
+          m[x][1] = max3(m[x][1], v.y, w.y);
+        }
+        moves |= m[x][0] > M[x][0] + kLag || m[x][1] > M[x][1] + kLag;
+      }
+      if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+        for (int x = 0; x < NB; ++x) {
+          float f[2], h[2];  // h: in the wide form, its root
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int y = 4; y <= 16; y <<= 1) m[x][e] = fmaxf(m[x][e], __shfl_xor_sync(0xffffffffu, m[x][e], y));
+            const float top = fmaxf(M[x][e], m[x][e]);
+            f[e] = M[x][e] == top ? 1.f : exp2_approx(M[x][e] - top);
+            if (WIDE) h[e] = M[x][e] == top ? 1.f : exp2_approx(0.5f * (M[x][e] - top));
+            M[x][e] = top;
+          }
+          l[x] = WIDE ? mul2(mul2(l[x], pair(h[0], h[1])), pair(h[0], h[1])) : mul2(l[x], pair(f[0], f[1]));
+          from[x] = pair(kLift - (M[x][0] == -INFINITY ? 0.f : M[x][0]), kLift - (M[x][1] == -INFINITY ? 0.f : M[x][1]));
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            o[i][x][0] *= f[0];
+            o[i][x][1] *= f[1];
+            o[i][x][2] *= f[0];
+            o[i][x][3] *= f[1];
+          }
+        }
+      }
+      // weights, as the columns of the second product: rows 2c, 2c + 1 of head g
+      uint32_t pw[2 * NS][NB];
+      float lv[2 * NS];
+      if (WIDE) {
+#pragma unroll
+        for (int j = 0; j < 2 * NS; ++j) lv[j] = tok[16 * (j >> 1) + 2 * (j & 1) + g0].y - kSumLift;
+      }
+#pragma unroll
+      for (int x = 0; x < NB; ++x)
+#pragma unroll
+        for (int j = 0; j < 2 * NS; ++j) {
+          const float2 e = both(add2(a[j][x], from[x]));
+          const float w0 = exp2_approx(e.x), w1 = exp2_approx(e.y);
+          l[x] = WIDE ? add2(l[x], pair(exp2_approx(e.x - lv[j]), exp2_approx(e.y - lv[j])))
+                      : fma2(pair(w0, w1), pair(inv[j], inv[j]), l[x]);
+          pw[j][x] = transpose8x8(Half16<__half>::pack(w0, w1));
+        }
+
+      failed = !farq::mbar_wait_bounded(bars + 8, parity, kAttnWaitNs);
+      clear(vbox, mask);
+      // values times weights: rows g and g + 8 of output tile y are values 16y + g and 16y + g + 8
+#pragma unroll
+      for (int t = 0; t < NS; ++t)
+#pragma unroll
+        for (int hh = 0; hh < NH; ++hh)
+#pragma unroll
+          for (int y = 0; y < NT / NH; y += 2) {
+            uint32_t w[4];
+            load_transposed(w, (vaddr + t * 16 * ROWB + hh * TOK * 128) ^ (y << 4));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              uint32_t a[4];
+              decode_pairs<E4M3>(w[2 * e], a[0], a[2]);
+              decode_pairs<E4M3>(w[2 * e + 1], a[1], a[3]);
+#pragma unroll
+              for (int x = 0; x < NB; ++x) mma16816(o[hh * 8 + y + e][x], a, pw[2 * t][x], pw[2 * t + 1][x]);
+            }
+          }
+      __syncwarp();  // the values and the factors are read
+      if (__any_sync(0xffffffffu, failed)) return false;
+      have = more;
+      if (more) copy(&v_map, 1);
+#pragma unroll
+      for (int t = 0; t < LT; ++t) mask[t] = cp_mask[t];
+    }
+    return false;
+  };
+  const bool wide = work(std::false_type{});
+  if (wide) {
+#pragma unroll
+    for (int x = 0; x < NB; ++x) l[x] = mul2(l[x], pair(kSumUp, kSumUp));
+    work(std::true_type{});
   }
   if (__any_sync(0xffffffffu, failed)) {
     // A copy did not arrive: wait (bounded) for those in flight, give NaN.
@@ -713,7 +750,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
       const int row = 2 * c + e + 8 * x;
       if (g == 0) {
         ml[warp * 2 * R + row] = M[x][e];
-        ml[warp * 2 * R + R + row] = sum;
+        ml[warp * 2 * R + R + row] = wide ? sum : sum * kSumUp;
       }
 #pragma unroll
       for (int y = 0; y < NT; ++y) {
@@ -723,6 +760,11 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     }
   // Join. out = sum_n w_n o_n / sum_n w_n l_n over the warps, w_n = 2^(M_n - max).
   constexpr int LPR = kAttnThreads / R;  // lanes of a head: 16 or 8
+  // total + w l, with w = 2^d
+  auto add_sum = [](float total, float l, float w, float d) {
+    const float h = exp2_approx(0.5f * d);
+    return d < kTwoSteps ? fmaf(h * l, h, total) : fmaf(w, l, total);
+  };
   auto finish = [&](float total) { return total == 0.f ? 0.f : 1.0f / total; };
   auto put_lse = [&](int row, float m, float total) {
     p.lse[((int64_t)b * p.Q.d + qi) * p.H.d * p.G + head0 + row] =
@@ -749,9 +791,11 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     const float from_all = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int n = 0; n < W; ++n) {
-      w[n] = exp2_approx(w[n] - from_all);
-      total = fmaf(w[n], ml[n * 2 * R + R + row], total);
+      const float d = w[n] - from_all;
+      w[n] = exp2_approx(d);
+      total = add_sum(total, ml[n * 2 * R + R + row], w[n], d);
     }
+    total *= 1.f / kSumUp;
     const float f = finish(total);
 #pragma unroll
     for (int k = 0; k < D / 4 / LPR; ++k) {
@@ -823,12 +867,13 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
 #pragma unroll
     for (int i = 0; i < MOST; ++i) {
       const uint32_t n = sub + i * LPR;
-      const float w = exp2_approx(top[i] - from_all);
-      total = fmaf(w, sum[i], total);
+      const float d = top[i] - from_all, w = exp2_approx(d);
+      total = add_sum(total, sum[i], w, d);
       if (n < NW) all[n * R + row] = w;
     }
 #pragma unroll
     for (int y = 1; y < LPR; y <<= 1) total += __shfl_xor_sync(0xffffffffu, total, y);
+    total *= 1.f / kSumUp;
     if (sub == 0) {
       fin[row] = finish(total);
       if (p.lse && rank == 0 && row < rows) put_lse(row, m, total);

@@ -1,0 +1,89 @@
+"""dsa_paged_attention at the ends of its inputs' ranges, against the plain
+implementation in 64 bits (oracle/kv_oracle.py).
+
+Tolerances: as in test_dsa_attention_gpu.py (u = 2^-24), with value scales
+between 2^-40 and 2^128 instead of near 1:
+  exponent log2 of a value scale is off by 2 of its last places, 4u * 128; the
+           sums score + log2(vs), - maximum and - log2(vs) round three times, u
+           * (|score| + 128) each; the maximum's own rounding cancels. Together
+           with the score's factor at most 10u * (|score| + 128).
+  sums     a rescaling of the denominator in two steps adds 2^-20; there is at
+           most one for every 32 tokens, and one in the join.
+  lse      the maximum and the logarithm of the sum may reach 128 + |lse| each and
+           cancel: 4u * (|lse| + 256).
+"""
+import math
+
+import pytest
+import torch
+
+from oracle import kv_oracle as R
+from flagos_kernelgen_72h_shanghai_2026_b200 import dsa_paged_attention, paged_kv_quant_write
+from test_dsa_attention_gpu import BF16, E4M3, INT8, U, dev, inputs, run  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def check(out, lse, r, D, qmax):
+    score = (D + 16) * 2 * U * r["score"] + 10 * U * (r["score"] + 128) + 2.0 ** -21
+    steps = (r["n"] / 32 + 2) * 2.0 ** -20
+    rel = 2.0 ** -11 + 2.0 ** -20 + 2 * score + (r["n"] / 16 + 2) * 17 * 2 * U + steps
+    floor = r["n"] * 2.0 ** -31 * qmax * r["top"]
+    tol = rel[..., None] * r["size"] + floor[..., None]
+    g, half = out.cpu().double(), torch.finfo(out.dtype).eps / 2
+    assert torch.equal(g.isnan(), r["out"].isnan())
+    off = ((g - r["out"]).abs() - half * (r["out"].abs() + tol) - tol).nan_to_num(-1.0)
+    assert float(off.max()) <= 0, f"out is off by {float(off.max()):.3g} more than allowed"
+    x, empty = lse.cpu().double(), r["lse"] == -math.inf
+    assert torch.equal(x == -math.inf, empty) and torch.equal(x.isnan(), r["lse"].isnan())
+    tol = score + 2.0 ** -20 + (r["n"] / 16 + 20) * U + 4 * U * (r["lse"].abs() + 256).nan_to_num(posinf=0.0) + steps
+    off = ((x - r["lse"]).abs() - tol)[~empty].nan_to_num(-1.0)
+    assert off.numel() == 0 or float(off.max()) <= 0, f"lse is off by {float(off.max()):.3g} more than allowed"
+
+
+# B, Q, K, G, D, block_size: a CTA alone (rows enough), and clusters of two to eight
+SHAPES = [(2, 3, 6, 4, 128, 32), (16, 4, 4, 16, 64, 64), (1, 1, 40, 4, 64, 64), (1, 1, 24, 16, 128, 64),
+          (2, 2, 8, 16, 256, 32), (1, 1, 8, 1, 256, 64)]
+
+
+# ------------------------------------------------------ value scales far apart
+def test_one_huge_value_among_zeros(dev):
+    """Written by the cache's own write: 31 value vectors of zeros (scale 1e-12) and one of 3e30, equal scores."""
+    H, D, bs = 1, 64, 32
+    k, v = torch.zeros(1, bs, H, D, dtype=BF16, device=dev), torch.zeros(1, bs, H, D, dtype=BF16, device=dev)
+    v[0, 3] = 3e30
+    cache = tuple(t.to(dev) for t in (torch.zeros(1, H, bs, D).to(E4M3), torch.zeros(1, H, bs),
+                                      torch.zeros(1, H, bs, D).to(E4M3), torch.zeros(1, H, bs)))
+    zero = torch.zeros(1, 1, dtype=torch.int32, device=dev)
+    paged_kv_quant_write(k, v, *cache, zero, torch.arange(bs, dtype=torch.int32, device=dev)[None])
+    q = torch.ones(1, 1, 1, D, dtype=BF16, device=dev)
+    out, lse = torch.zeros_like(q), torch.zeros(1, 1, 1, device=dev)
+    dsa_paged_attention(q, *cache, zero[None, None], zero[None, None], zero + bs - 1, zero[0] + bs, out, lse, 1.0)
+    want = float(v[0, 3, 0, 0]) / bs
+    # out: the code is exact (448), its scale rounded (u), the weight 2^-11 and the bound's 2^-14 of exponents
+    assert abs(float(lse) - math.log(bs)) <= 4 * U * 260 + 2.0 ** -19
+    assert ((out.double().cpu() - want).abs() <= want * (2.0 ** -8 + 2.0 ** -10)).all()
+
+
+@pytest.mark.parametrize("how", ["spread", "rising", "falling", "first", "last"])
+@pytest.mark.parametrize("code", [E4M3, INT8])
+@pytest.mark.parametrize("B,Q,K,G,D,bs", SHAPES, ids=str)
+def test_value_scales_far_apart(dev, B, Q, K, G, D, bs, code, how):
+    """Value scales from the least (1e-12) to 2^118: in no order, with the position, at one token alone."""
+    g, table, P, c, q, blocks, pages, pos, lens = inputs(60 + K, B=B, Q=Q, G=G, D=D, bs=bs, K=K, NB=K, code=code)
+    blocks = torch.arange(K).expand(B, 2, Q, K).int().contiguous()
+    pages = table[:, None, None, :].expand(B, 2, Q, K).contiguous()
+    n = K * bs
+    at = torch.arange(n).view(K, 1, bs)
+    for b in range(B):
+        if how == "spread":
+            ex = torch.randint(-39, 119, (K, 2, bs), generator=g).float()
+        elif how in ("rising", "falling"):
+            ex = -39 + 157 * at.expand(K, 2, bs).float() / (n - 1)
+            ex = ex if how == "rising" else ex.flip(0, 2)
+        else:
+            ex = torch.where(at == (0 if how == "first" else n - 1), 118.0, -40.0).expand(K, 2, bs)
+        c[3][table[b].long()] = torch.exp2(ex).clamp(min=R.MIN_SCALE)
+    r = R.dsa_paged_attention_ref(q, *c, blocks, pages, pos, lens, 0.1)
+    out, lse = run(dev, q, c, blocks, pages, pos, lens, 0.1)
+    check(out, lse, r, D, R.QMAX[code])
