@@ -23,6 +23,8 @@
 // 2^(a_t - M - log2(vs_t)) from then on, times 2^24 (a row's l lies between 2^-122
 // and 2^85: a term 2^-28 of the least one still counts), and l is multiplied by
 // powers of two that may themselves be too small in two steps, here and in the join.
+// It does the same from a value scale on that is not finite: such a token enters a_t
+// and l as if its scale were 1, and its weight in the second product is NaN.
 //
 // Precision: q is brought to fp16 by one power of two for all heads of a CTA, the
 // largest value in [2^14, 2^15): bf16 values lose bits only 2^-28 below it.
@@ -394,16 +396,20 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
   };
   float qs = 0.f;  // softmax_scale * log2(e) over the factor of the queries
   // Factors of this lane's tokens: of their scores, the exponent and the
-  // inverse of their value scales. True if one of them has a scale above kWide.
-  auto factors = [&] {
+  // inverse of their value scales (in the wide form, what makes their weights NaN).
+  // True if one of them has a scale above kWide, or one that is NaN.
+  auto factors = [&](auto is_wide) {
+    constexpr bool WIDE = decltype(is_wide)::value;
     bool above = false;
 #pragma unroll
     for (int t = 0; t < LT; ++t) {
       const float ks = scales[32 * t + lane];
       float vs = scales[TOK + 32 * t + lane];
       vs = vs < kMinScale ? kMinScale : vs;
-      above |= vs > kWide;
-      tok[32 * t + lane] = make_float4(ks * qs, __log2f(vs), rcp_approx(vs), 0.f);
+      above |= !(vs <= kWide);
+      const bool finite = vs <= 3.4028235e38f;
+      tok[32 * t + lane] = WIDE ? make_float4(ks * qs, finite ? __log2f(vs) : 0.f, finite ? 0.f : vs - vs, 0.f)
+                                : make_float4(ks * qs, __log2f(vs), rcp_approx(vs), 0.f);
     }
     return above;
   };
@@ -556,7 +562,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     for (bool again = WIDE; have; parity ^= 1) {
       // this chunk's factors, the next chunk's addresses
       asm volatile("cp.async.wait_all;" ::: "memory");
-      const bool above = factors();
+      const bool above = factors(is_wide);
       if (more && !again) prepare();
       again = false;
       // a wait that runs out ends the loop before the next copy
@@ -618,7 +624,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
       // exponents of heads 2c, 2c + 1. M moves when a lane sees a value well above
       // it; until then nothing has to be exchanged between lanes.
       f32x2 a[2 * NS][NB];
-      float inv[2 * NS], m[NB][2];
+      float inv[2 * NS], m[NB][2];  // inv: in the wide form NaN or 0, added to the weights
       bool partial = false;
 #pragma unroll
       for (int t = 0; t < LT; ++t) partial |= mask[t] != 0xffffffffu;
@@ -688,7 +694,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
           const float w0 = exp2_approx(e.x), w1 = exp2_approx(e.y);
           l[x] = WIDE ? add2(l[x], pair(exp2_approx(e.x - lv[j]), exp2_approx(e.y - lv[j])))
                       : fma2(pair(w0, w1), pair(inv[j], inv[j]), l[x]);
-          pw[j][x] = transpose8x8(Half16<__half>::pack(w0, w1));
+          pw[j][x] = transpose8x8(Half16<__half>::pack(WIDE ? w0 + inv[j] : w0, WIDE ? w1 + inv[j] : w1));
         }
 
       failed = !farq::mbar_wait_bounded(bars + 8, parity, kAttnWaitNs);

@@ -47,7 +47,9 @@ def dsa_paged_attention(q: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.T
     none, one that occurs twice counts twice. q_pos [B, Q] and kv_lens [B] as
     in the selection. ``lse`` [B, Q, Hq] fp32, or None, gets the natural
     logarithm of the softmax's denominator. A row without a token, and a
-    padded one (negative position), has out = 0 and lse = -inf.
+    padded one (negative position), has out = 0 and lse = -inf. A row that sees
+    a value vector stored with a NaN or an infinity has out = NaN and the lse of
+    its scores.
 
     D is 64, 128 or 256; block_size is 8 to 65536."""
     if L._fast is not None:

@@ -157,7 +157,9 @@ typedef struct dsa_kv_copy_args {
  * out may be q itself. A copy that has not arrived after two seconds ends its
  * row: the outputs become NaN.
  * v_scale is positive; one below 1e-12, the least that a write leaves, counts
- * as 1e-12.
+ * as 1e-12. One that is NaN (a vector that held a NaN or an infinity) or infinite
+ * makes out NaN in the rows that see its token; lse, which holds no values, is the
+ * same as with any other scale.
  * D is 64, 128 or 256, block_size >= 8.
  */
 typedef struct dsa_kv_attn_args {

@@ -87,3 +87,38 @@ def test_value_scales_far_apart(dev, B, Q, K, G, D, bs, code, how):
     r = R.dsa_paged_attention_ref(q, *c, blocks, pages, pos, lens, 0.1)
     out, lse = run(dev, q, c, blocks, pages, pos, lens, 0.1)
     check(out, lse, r, D, R.QMAX[code])
+
+
+@pytest.mark.parametrize("code", [E4M3, INT8])
+@pytest.mark.parametrize("B,Q,K,G,D,bs", SHAPES, ids=str)
+def test_lse_holds_no_values(dev, B, Q, K, G, D, bs, code):
+    """Value vectors with a NaN or an infinity, stored by the write with the scale NaN: out is NaN in the rows that see
+    them, lse what the scores give. The same with a scale of infinity."""
+    g, table, P, c, q, blocks, pages, pos, lens = inputs(70 + K, B=B, Q=Q, G=G, D=D, bs=bs, K=K, NB=K + 2, code=code)
+    v = torch.randn(B, 3, 2, D, generator=g).to(BF16)
+    v[0, 0, 0, 5], v[0, 1, 1, D - 1], v[-1, 2, 0] = math.nan, math.inf, -math.inf
+    at = torch.tensor([[0, bs + 1, (K + 2) * bs - Q]]).expand(B, 3).int().contiguous()
+    cd = tuple(t.to(dev) for t in c)
+    paged_kv_quant_write(torch.zeros_like(v).to(dev), v.to(dev), *cd, table.to(dev), at.to(dev))
+    c = [t.cpu() for t in cd]
+    r = R.dsa_paged_attention_ref(q, *c, blocks, pages, pos, lens, 0.1)
+    out, lse = run(dev, q, c, blocks, pages, pos, lens, 0.1)
+    assert r["out"].isnan().any() and not r["lse"].isnan().any()
+    assert torch.equal(out.cpu().isnan(), r["out"].isnan())
+    r["out"], r["size"] = r["out"].nan_to_num(0.0), r["size"].nan_to_num(0.0)
+    r["top"] = r["top"].nan_to_num(0.0)
+    check(out.nan_to_num(0.0), lse, r, D, R.QMAX[code])
+    c[3] = c[3].nan_to_num(math.inf)
+    inf_out, inf_lse = run(dev, q, c, blocks, pages, pos, lens, 0.1)
+    assert torch.equal(inf_out.isnan(), out.isnan()) and torch.equal(inf_lse, lse)
+
+
+def test_all_values_without_a_scale(dev):
+    """Every value scale NaN: no finite value scale to hold the maximum."""
+    _, _, _, c, q, blocks, pages, pos, lens = inputs(71)
+    c[3] = torch.full_like(c[3], math.nan)
+    r = R.dsa_paged_attention_ref(q, *c, blocks, pages, pos, lens, 0.1)
+    out, lse = run(dev, q, c, blocks, pages, pos, lens, 0.1)
+    r["out"], r["size"], r["top"] = (torch.zeros_like(r[k]) for k in ("out", "size", "top"))
+    assert out.isnan().all()
+    check(torch.zeros_like(out), lse, r, 128, 448.0)
