@@ -75,7 +75,12 @@ constexpr int kAttnWarps = 4;      // warps of a CTA
 constexpr int kAttnThreads = 32 * kAttnWarps;
 constexpr int kMaxCluster = 8;
 constexpr float kLift = 6.0f;      // weights are 2^(a - M + kLift)
-constexpr float kLag = 8.0f;       // M is moved when a maximum exceeds it by more
+// The kernel holds M - kLift as it is rounded, and takes all differences from that: from
+// 2^24 on kLift is below M's last place. It is moved where a maximum is at least the
+// rounded (M - kLift) + kLift + kLag, so that no weight is above 2^14: a maximum that is
+// larger than the sum is not smaller than the sum rounded. (Moved where M + kLag was
+// exceeded, values 16 above an M of 2^26 stayed, and 2^(16 + kLift) is no fp16 number.)
+constexpr float kLag = 8.0f;
 constexpr float kWide = 4294967296.0f;  // value scales up to it: 1 / vs brings every term of l that counts back
 constexpr float kSumLift = 24.0f;       // l is 2^kSumLift times its value from there on, and in the join
 constexpr float kSumUp = 16777216.0f;   // 2^kSumLift
@@ -118,7 +123,7 @@ struct AttnSmem {
   static constexpr size_t tok = ring + W * region;                // [W][TOK] factors of a chunk's tokens
   static constexpr size_t scales = tok + (size_t)W * TOK * 16;    // [W][2][TOK]
   static constexpr size_t bars = scales + (size_t)W * 2 * TOK * 4;  // [W][2]
-  static constexpr size_t ml = bars + (size_t)W * 2 * 8;          // [W][2][R] maxima and sums
+  static constexpr size_t ml = bars + (size_t)W * 2 * 8;          // [W][2][R] maxima less kLift, and sums
   static constexpr size_t fin = ml + (size_t)W * 2 * R * 4;          // [R] 1 / l
   static constexpr bool q_in_smem = D >= 128 && NB == 2;             // where the output fills the registers
   static constexpr size_t qf = fin + R * 4;
@@ -529,17 +534,17 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
   }
 
   float o[NT][NB][4];
-  float M[NB][2];  // of heads 2c, 2c + 1 (+ 8x)
-  f32x2 l[NB], from[NB];  // sums of weights; kLift - M
+  float ref[NB][2];  // M - kLift of heads 2c, 2c + 1 (+ 8x)
+  f32x2 l[NB], from[NB];  // sums of weights; -ref
 #pragma unroll
   for (int x = 0; x < NB; ++x) {
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][x][e] = 0.f;
-    M[x][0] = M[x][1] = -INFINITY;
+    ref[x][0] = ref[x][1] = -INFINITY;
     l[x] = 0;
-    from[x] = pair(kLift, kLift);
+    from[x] = 0;
   }
   bool failed = false;
 
@@ -653,7 +658,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
           m[x][0] = max3(m[x][0], v.x, w.x);
           m[x][1] = max3(m[x][1], v.y, w.y);
         }
-        moves |= m[x][0] > M[x][0] + kLag || m[x][1] > M[x][1] + kLag;
+        moves |= m[x][0] >= ref[x][0] + (kLift + kLag) || m[x][1] >= ref[x][1] + (kLift + kLag);
       }
       if (__any_sync(0xffffffffu, moves)) {
 #pragma unroll
@@ -663,13 +668,13 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
           for (int e = 0; e < 2; ++e) {
 #pragma unroll
             for (int y = 4; y <= 16; y <<= 1) m[x][e] = fmaxf(m[x][e], __shfl_xor_sync(0xffffffffu, m[x][e], y));
-            const float top = fmaxf(M[x][e], m[x][e]);
-            f[e] = M[x][e] == top ? 1.f : exp2_approx(M[x][e] - top);
-            if (WIDE) h[e] = M[x][e] == top ? 1.f : exp2_approx(0.5f * (M[x][e] - top));
-            M[x][e] = top;
+            const float top = fmaxf(ref[x][e], m[x][e] - kLift);
+            f[e] = ref[x][e] == top ? 1.f : exp2_approx(ref[x][e] - top);
+            if (WIDE) h[e] = ref[x][e] == top ? 1.f : exp2_approx(0.5f * (ref[x][e] - top));
+            ref[x][e] = top;
           }
           l[x] = WIDE ? mul2(mul2(l[x], pair(h[0], h[1])), pair(h[0], h[1])) : mul2(l[x], pair(f[0], f[1]));
-          from[x] = pair(kLift - (M[x][0] == -INFINITY ? 0.f : M[x][0]), kLift - (M[x][1] == -INFINITY ? 0.f : M[x][1]));
+          from[x] = pair(ref[x][0] == -INFINITY ? 0.f : -ref[x][0], ref[x][1] == -INFINITY ? 0.f : -ref[x][1]);
 #pragma unroll
           for (int i = 0; i < NT; ++i) {
             o[i][x][0] *= f[0];
@@ -755,7 +760,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
       for (int y = 4; y <= 16; y <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, y);
       const int row = 2 * c + e + 8 * x;
       if (g == 0) {
-        ml[warp * 2 * R + row] = M[x][e];
+        ml[warp * 2 * R + row] = ref[x][e];
         ml[warp * 2 * R + R + row] = wide ? sum : sum * kSumUp;
       }
 #pragma unroll
@@ -774,7 +779,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
   auto finish = [&](float total) { return total == 0.f ? 0.f : 1.0f / total; };
   auto put_lse = [&](int row, float m, float total) {
     p.lse[((int64_t)b * p.Q.d + qi) * p.H.d * p.G + head0 + row] =
-        total == 0.f ? -INFINITY : (m - kLift + log2f(total)) * 0.69314718055994531f;
+        total == 0.f ? -INFINITY : (m + log2f(total)) * 0.69314718055994531f;
   };
   auto store = [&](int row, int f4, const float4& acc, float f) {
     uint2 v;

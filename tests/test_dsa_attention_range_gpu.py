@@ -122,3 +122,36 @@ def test_all_values_without_a_scale(dev):
     r["out"], r["size"], r["top"] = (torch.zeros_like(r[k]) for k in ("out", "size", "top"))
     assert out.isnan().all()
     check(torch.zeros_like(out), lse, r, 128, 448.0)
+
+
+# ---------------------------------------------------------------- large scores
+LN2 = 0.6931471805599453  # times log2(e) in fp32: 1
+
+
+@pytest.mark.parametrize("above", [0, 1])
+@pytest.mark.parametrize("e", [22, 23, 24, 25, 26, 27, 28])
+def test_scores_a_few_places_apart(dev, e, above):
+    """Scores of 2^e in units of ln 2, one to eight of their last places apart, the larger ones in a warp's second chunk.
+    Every step up to the weights is exact, and these are powers of two: out is off by its own rounding, the sums' and
+    the exponentials' (2^-20 at most); a weight below 2^-20 may go."""
+    ulp = 2.0 ** (e - 23)
+    B, Q, H, K, D, bs = 1, 128, 4, 8, 64, 64
+    g, table, P, c, _, _, _, pos, lens = inputs(80, B=B, Q=Q, H=H, G=1, D=D, bs=bs, K=K, NB=K, code=INT8)
+    blocks = torch.arange(K).expand(B, H, Q, K).int().contiguous()
+    pages = table[:, None, None, :].expand(B, H, Q, K).contiguous()
+    pos[:] = K * bs - 1
+    q = torch.zeros(B, Q, H, D, dtype=BF16)
+    q[..., 0], q[..., 1] = 2.0 ** (e - 6), ulp
+    for delta in (1, 2, 4, 8):
+        if delta * ulp > 64:
+            continue
+        kc, vc = torch.zeros(P, H, bs, D, dtype=torch.int8), torch.ones(P, H, bs, D, dtype=torch.int8)
+        kc[..., 0], kc[..., 1] = 64, above
+        high = table[0, 4:].long()
+        kc[high, :, 9, 1] = above + delta
+        vc[high, :, 9] = 3
+        one = torch.ones(P, H, bs)
+        out, _ = run(dev, q, (kc, one, vc, one), blocks, pages, pos, lens, LN2)
+        w = 4 * 2.0 ** (delta * ulp)
+        want = (K * bs - 4 + 3 * w) / (K * bs - 4 + w)
+        assert abs(out.float() - want).max() <= want * (2.0 ** -8 + 2.0 ** -18) + 512 * 2.0 ** -20, (delta, want)
