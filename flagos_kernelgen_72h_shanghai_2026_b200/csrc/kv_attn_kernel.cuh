@@ -27,7 +27,9 @@
 // and l as if its scale were 1, and its weight in the second product is NaN.
 //
 // Precision: q is brought to fp16 by one power of two for all heads of a CTA, the
-// largest value in [2^14, 2^15): bf16 values lose bits only 2^-28 below it.
+// largest value in [2^14, 2^15): bf16 values lose bits only 2^-28 below it. Where a
+// head's largest value is more than 2^8 below the CTA's, every head has a power of its
+// own, and all chunks go through the loop's second copy, which applies them.
 // Weights are fp16 too, times 2^6: 2^-11 relative (the output's own half step
 // is 2^-9 or 2^-12) down to 2^-20, with an absolute 2^-31 below. M lags behind
 // the maximum by up to 8 (a weight is at most 2^14), so that o is rescaled
@@ -123,7 +125,8 @@ struct AttnSmem {
   static constexpr size_t tok = ring + W * region;                // [W][TOK] factors of a chunk's tokens
   static constexpr size_t scales = tok + (size_t)W * TOK * 16;    // [W][2][TOK]
   static constexpr size_t bars = scales + (size_t)W * 2 * TOK * 4;  // [W][2]
-  static constexpr size_t ml = bars + (size_t)W * 2 * 8;          // [W][2][R] maxima less kLift, and sums
+  // [W][2][R] maxima less kLift, and sums; until then the heads' own powers of two
+  static constexpr size_t ml = bars + (size_t)W * 2 * 8;
   static constexpr size_t fin = ml + (size_t)W * 2 * R * 4;          // [R] 1 / l
   static constexpr bool q_in_smem = D >= 128 && NB == 2;             // where the output fills the registers
   static constexpr size_t qf = fin + R * 4;
@@ -400,9 +403,11 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     }
   };
   float qs = 0.f;  // softmax_scale * log2(e) over the factor of the queries
+  // Value scales above it take the wide form of the loop: all, where heads have powers of their own.
+  float limit = kWide;
   // Factors of this lane's tokens: of their scores, the exponent and the
   // inverse of their value scales (in the wide form, what makes their weights NaN).
-  // True if one of them has a scale above kWide, or one that is NaN.
+  // True if one of them has a scale above the limit, or one that is NaN.
   auto factors = [&](auto is_wide) {
     constexpr bool WIDE = decltype(is_wide)::value;
     bool above = false;
@@ -411,7 +416,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
       const float ks = scales[32 * t + lane];
       float vs = scales[TOK + 32 * t + lane];
       vs = vs < kMinScale ? kMinScale : vs;
-      above |= !(vs <= kWide);
+      above |= !(vs <= limit);
       const bool finite = vs <= 3.4028235e38f;
       tok[32 * t + lane] = WIDE ? make_float4(ks * qs, finite ? __log2f(vs) : 0.f, finite ? 0.f : vs - vs, 0.f)
                                 : make_float4(ks * qs, __log2f(vs), rcp_approx(vs), 0.f);
@@ -470,28 +475,54 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     for (int t = 0; t < LT; ++t) mask[t] = cp_mask[t];
   }
 
-  // In fp16, times the power of two that brings the CTA's largest finite value
-  // into [2^14, 2^15).
+  // In fp16, times the power of two that brings the CTA's largest finite value,
+  // or each head's, into [2^14, 2^15).
   uint32_t qf[QSMEM ? 1 : D / 16][NB][2];
   {
     // The largest magnitude is the largest of the bits without the sign; one
     // that is not finite is left out, value by value.
-    uint32_t bits = 0;
+    constexpr int MANTISSA = Half16<T>::kInf == 0x7f80u ? 7 : 10;  // bits
+    uint32_t head[NB], all, low;  // largest of a lane's (then of a head's), of all; the least of those that are not 0
+    auto ends = [&] {
+      all = 0;
+      low = 0xffffu;
 #pragma unroll
-    for (int x = 0; x < NB; ++x)
+      for (int x = 0; x < NB; ++x) {
+        all = max(all, head[x]);
+        low = min(low, head[x] - 1);
+      }
+      all = __reduce_max_sync(0xffffffffu, all);
+      low = __reduce_min_sync(0xffffffffu, low) + 1;
+    };
+    auto largest = [&](auto all_finite) {
 #pragma unroll
-      for (int hh = 0; hh < NH; ++hh)
+      for (int x = 0; x < NB; ++x) {
+        uint32_t bits = 0;
 #pragma unroll
-        for (int i = 0; i < NU * 2; ++i) {
-          const uint4& v = raw[x][hh][i];
-          bits = __vmaxu2(bits, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
-                                         __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
-        }
-    bits = max(bits & 0xffffu, bits >> 16);
-    bits = __reduce_max_sync(0xffffffffu, bits);
-    float most = Half16<T>::unpack(bits).x;
-    if (bits >= Half16<T>::kInf) {
-      most = 0.f;
+        for (int hh = 0; hh < NH; ++hh)
+#pragma unroll
+          for (int i = 0; i < NU * 2; ++i) {
+            const uint4& v = raw[x][hh][i];
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t u = w[e] & 0x7fff7fffu;
+              if (!decltype(all_finite)::value) {
+                if ((u & 0xffffu) >= Half16<T>::kInf) u &= 0xffff0000u;
+                if ((u >> 16) >= Half16<T>::kInf) u &= 0xffffu;
+              }
+              bits = __vmaxu2(bits, u);
+            }
+          }
+        head[x] = max(bits & 0xffffu, bits >> 16);
+      }
+      ends();
+    };
+    auto exponent = [](uint32_t bits) {
+      return max((int)(__float_as_uint(Half16<T>::unpack(bits).x) >> 23) - 127, -100);
+    };
+    auto power = [](int e) { return __uint_as_float((uint32_t)(e + 127) << 23); };
+    auto convert = [&](const float (&up)[NB]) {
 #pragma unroll
       for (int x = 0; x < NB; ++x)
 #pragma unroll
@@ -501,35 +532,51 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
             float f[8];
             unpack8<T>(raw[x][hh][i], f);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[e]) <= 3.4e38f ? fabsf(f[e]) : 0.f);
-          }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    }
-    const int ex = max((int)(__float_as_uint(most) >> 23) - 127, -100);
-    const float up = most > 0.f ? __uint_as_float((uint32_t)(14 - ex + 127) << 23) : 1.f;
-    qs = p.scale / up;
-#pragma unroll
-    for (int x = 0; x < NB; ++x)
-#pragma unroll
-      for (int hh = 0; hh < NH; ++hh)
-#pragma unroll
-        for (int i = 0; i < NU * 2; ++i) {
-          float f[8];
-          unpack8<T>(raw[x][hh][i], f);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int ks = (hh * NU * 2 + i) * 2 + e;
-            const uint32_t b0 = Half16<__half>::pack(f[4 * e] * up, f[4 * e + 1] * up);
-            const uint32_t b1 = Half16<__half>::pack(f[4 * e + 2] * up, f[4 * e + 3] * up);
-            if (QSMEM) {
-              if (warp == 0) *reinterpret_cast<uint2*>(smem + L::qf + ((ks * NB + x) * 32 + lane) * 8) = make_uint2(b0, b1);
-            } else {
-              qf[QSMEM ? 0 : ks][x][0] = b0;
-              qf[QSMEM ? 0 : ks][x][1] = b1;
+            for (int e = 0; e < 2; ++e) {
+              const int ks = (hh * NU * 2 + i) * 2 + e;
+              const uint32_t b0 = Half16<__half>::pack(f[4 * e] * up[x], f[4 * e + 1] * up[x]);
+              const uint32_t b1 = Half16<__half>::pack(f[4 * e + 2] * up[x], f[4 * e + 3] * up[x]);
+              if (QSMEM) {
+                if (warp == 0)
+                  *reinterpret_cast<uint2*>(smem + L::qf + ((ks * NB + x) * 32 + lane) * 8) = make_uint2(b0, b1);
+              } else {
+                qf[QSMEM ? 0 : ks][x][0] = b0;
+                qf[QSMEM ? 0 : ks][x][1] = b1;
+              }
             }
           }
-        }
+    };
+    // More than 2^8 apart? Lanes first, and where they are, the heads, which four lanes hold.
+    auto apart = [&] { return (all >> MANTISSA) > (low >> MANTISSA) + 8; };
+    largest(std::true_type{});
+    if (all >= Half16<T>::kInf || apart()) {
+      largest(std::false_type{});
+#pragma unroll
+      for (int x = 0; x < NB; ++x)
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) head[x] = max(head[x], __shfl_xor_sync(0xffffffffu, head[x], o));
+      ends();
+    }
+    float up[NB];
+    if (apart()) {
+      limit = -1.f;
+      // A head's own power is 2^(14 - ex); its scores are taken times 2^(ex - least), at
+      // most 2^96 (a score before the scales is below 2^32), and qs times the rest.
+      const int least = max(exponent(all) - 96, 0);
+#pragma unroll
+      for (int x = 0; x < NB; ++x) {
+        const int ex = exponent(head[x]);
+        up[x] = power(14 - ex);
+        if (c == 0) reinterpret_cast<float*>(smem + L::ml)[warp * 2 * R + g + 8 * x] = ldexpf(1.f, ex - least);
+      }
+      qs = p.scale * power(least - 14);
+      convert(up);
+    } else {
+#pragma unroll
+      for (int x = 0; x < NB; ++x) up[x] = all != 0 ? power(14 - exponent(all)) : 1.f;
+      qs = p.scale / up[0];
+      convert(up);
+    }
     if (QSMEM) __syncthreads();
   }
 
@@ -559,7 +606,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
   uint8_t* const vbox = ring + L::box;
   uint32_t parity = 0;
   // Works on chunks until none is left, or, where it is not `wide`, one holds a
-  // value scale above kWide: then true, and the wide copy begins with that chunk
+  // value scale above the limit: then true, and the wide copy begins with that chunk
   // anew, its keys still in their box and the next chunk's addresses at hand. One
   // loop with both forms of the sums was 4 % slower (1024 rows x 16 heads x 2048 tokens).
   auto work = [&](auto is_wide) -> bool {
@@ -629,17 +676,29 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
       // exponents of heads 2c, 2c + 1. M moves when a lane sees a value well above
       // it; until then nothing has to be exchanged between lanes.
       f32x2 a[2 * NS][NB];
-      float inv[2 * NS], m[NB][2];  // inv: in the wide form NaN or 0, added to the weights
+      float inv[2 * NS], m[NB][2];
       bool partial = false;
 #pragma unroll
       for (int t = 0; t < LT; ++t) partial |= mask[t] != 0xffffffffu;
+      auto factor = [&](int j) { return tok[16 * (j >> 1) + 2 * (j & 1) + g0]; };
+      if (WIDE) {  // the heads' own powers of two
+#pragma unroll
+        for (int x = 0; x < NB; ++x) {
+          const float2 own = reinterpret_cast<const float2*>(smem + L::ml)[warp * R + c + 4 * x];
+#pragma unroll
+          for (int t = 0; t < NS; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[t][x][e] *= e & 1 ? own.y : own.x;
+        }
+      }
 #pragma unroll
       for (int j = 0; j < 2 * NS; ++j) {
-        const float4 f = tok[16 * (j >> 1) + 2 * (j & 1) + g0];
+        const float4 f = factor(j);
         inv[j] = f.z;
 #pragma unroll
         for (int x = 0; x < NB; ++x)
-          a[j][x] = fma2(pair(sc[j >> 1][x][(j & 1) * 2], sc[j >> 1][x][(j & 1) * 2 + 1]), pair(f.x, f.x), pair(f.y, f.y));
+          a[j][x] =
+              fma2(pair(sc[j >> 1][x][(j & 1) * 2], sc[j >> 1][x][(j & 1) * 2 + 1]), pair(f.x, f.x), pair(f.y, f.y));
       }
       if (partial) {
 #pragma unroll
@@ -686,20 +745,22 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
       }
       // weights, as the columns of the second product: rows 2c, 2c + 1 of head g
       uint32_t pw[2 * NS][NB];
-      float lv[2 * NS];
-      if (WIDE) {
-#pragma unroll
-        for (int j = 0; j < 2 * NS; ++j) lv[j] = tok[16 * (j >> 1) + 2 * (j & 1) + g0].y - kSumLift;
-      }
 #pragma unroll
       for (int x = 0; x < NB; ++x)
 #pragma unroll
         for (int j = 0; j < 2 * NS; ++j) {
           const float2 e = both(add2(a[j][x], from[x]));
-          const float w0 = exp2_approx(e.x), w1 = exp2_approx(e.y);
-          l[x] = WIDE ? add2(l[x], pair(exp2_approx(e.x - lv[j]), exp2_approx(e.y - lv[j])))
-                      : fma2(pair(w0, w1), pair(inv[j], inv[j]), l[x]);
-          pw[j][x] = transpose8x8(Half16<__half>::pack(WIDE ? w0 + inv[j] : w0, WIDE ? w1 + inv[j] : w1));
+          float w0 = exp2_approx(e.x), w1 = exp2_approx(e.y);
+          if (WIDE) {
+            const float4 f = factor(j);
+            const float lv = f.y - kSumLift;
+            l[x] = add2(l[x], pair(exp2_approx(e.x - lv), exp2_approx(e.y - lv)));
+            w0 += f.z;  // 0 or NaN
+            w1 += f.z;
+          } else {
+            l[x] = fma2(pair(w0, w1), pair(inv[j], inv[j]), l[x]);
+          }
+          pw[j][x] = transpose8x8(Half16<__half>::pack(w0, w1));
         }
 
       failed = !farq::mbar_wait_bounded(bars + 8, parity, kAttnWaitNs);
@@ -734,7 +795,11 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
   const bool wide = work(std::false_type{});
   if (wide) {
 #pragma unroll
-    for (int x = 0; x < NB; ++x) l[x] = mul2(l[x], pair(kSumUp, kSumUp));
+    for (int x = 0; x < NB; ++x) {
+      l[x] = mul2(l[x], pair(kSumUp, kSumUp));
+      if (limit == kWide && c == 0) reinterpret_cast<float*>(smem + L::ml)[warp * 2 * R + g + 8 * x] = 1.f;
+    }
+    __syncwarp();
     work(std::true_type{});
   }
   if (__any_sync(0xffffffffu, failed)) {

@@ -19,7 +19,7 @@ import torch
 
 from oracle import kv_oracle as R
 from flagos_kernelgen_72h_shanghai_2026_b200 import dsa_paged_attention, paged_kv_quant_write
-from test_dsa_attention_gpu import BF16, E4M3, INT8, U, dev, inputs, run  # noqa: F401
+from test_dsa_attention_gpu import BF16, E4M3, FP16, INT8, U, dev, inputs, run  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -155,3 +155,27 @@ def test_scores_a_few_places_apart(dev, e, above):
         w = 4 * 2.0 ** (delta * ulp)
         want = (K * bs - 4 + 3 * w) / (K * bs - 4 + w)
         assert abs(out.float() - want).max() <= want * (2.0 ** -8 + 2.0 ** -18) + 512 * 2.0 ** -20, (delta, want)
+
+
+# ------------------------------------------------------- heads of unlike size
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("code", [E4M3, INT8])
+@pytest.mark.parametrize("B,Q,K,G,D,bs", [*SHAPES, (1, 2, 5, 40, 64, 48)], ids=str)
+def test_heads_of_unlike_size(dev, B, Q, K, G, D, bs, code, dtype):
+    """Query heads up to 2^230 (fp16: 2^24) apart that share a key head: each has the scores of its own size, also beside
+    heads of zeros and of values that are not finite."""
+    _, table, P, c, q, blocks, pages, pos, lens = inputs(90 + G, B=B, Q=Q, G=G, D=D, bs=bs, K=K, NB=K + 1, code=code)
+    most = 115 if dtype == BF16 else 12
+    ex = torch.tensor([0, -9, most, -most, 3, -17, most - 5, 0, 9, -3])[torch.arange(2 * G) % 10]
+    q = q.float() * torch.exp2(ex.float())[:, None]
+    q[..., 5 % (2 * G), :] = 0
+    if G > 2:
+        q[0, 0, 1, 3], q[0, 0, G + 1, 7] = math.nan, math.inf
+    q = q.to(dtype)
+    r = R.dsa_paged_attention_ref(q, *c, blocks, pages, pos, lens, 0.1)
+    out, lse = run(dev, q, c, blocks, pages, pos, lens, 0.1)
+    bad = ~q.isfinite().all(-1)
+    got_o, got_l = out.cpu(), lse.cpu()
+    assert got_o[bad].isnan().all()
+    ok = {k: v[~bad] for k, v in r.items()}
+    check(got_o[~bad], got_l[~bad], ok, D, R.QMAX[code])
