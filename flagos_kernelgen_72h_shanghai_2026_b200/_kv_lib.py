@@ -34,8 +34,9 @@ ERR_ALIGNMENT = 5
 ERR_UNSUPPORTED = 6
 ERR_CUDA = 7
 ERR_BAD_ARGS_SIZE = 8
+ERR_DEVICE_TIMEOUT = 9
 
-ABI_VERSION = 1
+ABI_VERSION = 2
 
 HALF_DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_FP16}
 GAMMA_DTYPES = {**HALF_DTYPES, torch.float32: DTYPE_FP32}
@@ -129,17 +130,20 @@ def load(path: Path | str | None = None) -> ctypes.CDLL:
                 "Build it with: python -m flagos_kernelgen_72h_shanghai_2026_b200._build"
             )
         lib = ctypes.CDLL(str(p))
-        for name, args in _LAUNCHES.items():
-            fn = getattr(lib, name)
-            fn.argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
-            fn.restype = ctypes.c_int
-        lib.dsa_kv_strerror.argtypes = [ctypes.c_int]
-        lib.dsa_kv_strerror.restype = ctypes.c_char_p
         lib.dsa_kv_abi_version.argtypes = []
         lib.dsa_kv_abi_version.restype = ctypes.c_int
         v = lib.dsa_kv_abi_version()
         if v != ABI_VERSION:
             raise RuntimeError(f"libdsa_kv.so ABI version {v} != expected {ABI_VERSION}; rebuild it")
+        for name, args in _LAUNCHES.items():
+            fn = getattr(lib, name)
+            fn.argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+            fn.restype = ctypes.c_int
+        lib.dsa_kv_attn_launch_status.argtypes = [ctypes.POINTER(AttnArgs), ctypes.c_void_p,
+                                                  ctypes.c_int32, ctypes.c_void_p]
+        lib.dsa_kv_attn_launch_status.restype = ctypes.c_int
+        lib.dsa_kv_strerror.argtypes = [ctypes.c_int]
+        lib.dsa_kv_strerror.restype = ctypes.c_char_p
         if path is None:
             _lib = lib
         return lib
@@ -158,12 +162,12 @@ def raise_status(op: str, status: int):
     raise ValueError(msg)
 
 
-def launch(op: str, entry: str, args, device: torch.device) -> None:
+def launch(op: str, entry: str, args, device: torch.device, *more) -> None:
     """Call a C entry point on the device's current stream; raise its error."""
     fn = getattr(load(), entry)
     with torch.cuda.device(device):
         stream = torch.cuda.current_stream(device).cuda_stream
-        st = fn(ctypes.byref(args), ctypes.c_void_p(stream))
+        st = fn(ctypes.byref(args), *more, ctypes.c_void_p(stream))
     if st != OK:
         raise_status(op, st)
 

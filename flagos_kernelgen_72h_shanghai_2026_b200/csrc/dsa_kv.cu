@@ -199,6 +199,7 @@ const char* dsa_kv_strerror(int status) {
     case DSA_KV_ERR_CUDA: return "a CUDA call failed";
     case DSA_KV_ERR_BAD_ARGS_SIZE:
       return "argument struct size mismatch (header and library differ) or reserved field not 0";
+    case DSA_KV_ERR_DEVICE_TIMEOUT: return "a bounded device-side wait ran out";
     default: return "unknown dsa_kv status";
   }
 }

@@ -86,12 +86,12 @@ int64_t max_clusters(const Variant& v, int dev, int n, int log_c) {
   return count;
 }
 
-int attn(const dsa_kv_attn_args_t* a, void* stream) {
+int attn(const dsa_kv_attn_args_t* a, int32_t* status, int32_t test_copies, void* stream) {
   if (!a) return DSA_KV_ERR_NULL_POINTER;
   if (a->struct_size != sizeof(*a)) return DSA_KV_ERR_BAD_ARGS_SIZE;
   const int bb = index_size(a->block_dtype), pb = index_size(a->page_dtype), ib = index_size(a->pos_dtype);
   if (!is_16bit(a->dtype) || !bb || !pb || !ib) return DSA_KV_ERR_BAD_DTYPE;
-  if (a->B < 0 || a->Q < 0 || a->G < 1 || a->K < 0) return DSA_KV_ERR_BAD_SHAPE;
+  if (a->B < 0 || a->Q < 0 || a->G < 1 || a->K < 0 || test_copies < 0 || test_copies == 1) return DSA_KV_ERR_BAD_SHAPE;
   int st = check_cache(a->cache, kCacheMapped);
   if (st != DSA_KV_OK) return st;
   const dsa_kv_cache_t& c = a->cache;
@@ -108,7 +108,7 @@ int attn(const dsa_kv_attn_args_t* a, void* stream) {
   if ((st = check_dense(a->out, a->B, a->Q, c.H * a->G, true)) != DSA_KV_OK) return st;
   if (!a->q_pos || !a->kv_lens || (a->K > 0 && (!a->blocks || !a->pages))) return DSA_KV_ERR_NULL_POINTER;
   if (!aligned(a->blocks, bb) || !aligned(a->pages, pb) || !aligned(a->q_pos, ib) || !aligned(a->kv_lens, ib) ||
-      !aligned(a->lse, 4))
+      !aligned(a->lse, 4) || !aligned(status, 4))
     return DSA_KV_ERR_ALIGNMENT;
 
   const int64_t tiles = a->B * a->Q * c.H * MT;
@@ -200,6 +200,8 @@ int attn(const dsa_kv_attn_args_t* a, void* stream) {
   p.bs = (int32_t)c.block_size;
   p.cluster = (uint32_t)cluster;
   p.early = early;
+  p.status = status;
+  p.give_up = test_copies < 1 << 30 ? (uint32_t)test_copies : 0;
   p.log_pieces = log_pieces;
   p.box_bytes = (uint32_t)(box_rows * (c.D == 64 ? 64 : 128));
   p.block_bytes = bb;
@@ -216,4 +218,11 @@ int attn(const dsa_kv_attn_args_t* a, void* stream) {
 
 }  // namespace kv
 
-extern "C" int dsa_kv_attn_launch(const dsa_kv_attn_args_t* a, void* stream) { return kv::attn(a, stream); }
+extern "C" {
+
+int dsa_kv_attn_launch(const dsa_kv_attn_args_t* a, void* stream) { return kv::attn(a, nullptr, 0, stream); }
+int dsa_kv_attn_launch_status(const dsa_kv_attn_args_t* a, int32_t* status, int32_t test_copies, void* stream) {
+  return kv::attn(a, status, test_copies, stream);
+}
+
+}  // extern "C"

@@ -110,6 +110,8 @@ struct AttnParams {
   int32_t block_bytes, page_bytes, pos_bytes;
   uint32_t cluster;     // CTAs that share a row's tokens
   bool early;           // the next launch fits beside this one
+  int32_t* status;      // may be null
+  uint32_t give_up;     // test only: copies after which a row's first warp takes its next wait as run out
   float scale;          // softmax_scale * log2(e)
 };
 
@@ -377,7 +379,9 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     cp_page = __shfl_sync(0xffffffffu, pc_page, first + lane);
     cp_off = __shfl_sync(0xffffffffu, pc_off, first + lane);
   };
-  uint32_t started = 0;  // copies so far: the i-th fills box i % 2
+  // Copies so far: the i-th fills box i % 2. Warps other than a row's first count
+  // from 2^30, which p.give_up never is.
+  uint32_t started = wid == 0 ? 0 : 1u << 30;
   auto copy = [&](const CUtensorMap* map, int s) {
     const uint32_t bar = bars + 8 * s;
     ++started;
@@ -403,8 +407,10 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     }
   };
   float qs = 0.f;  // softmax_scale * log2(e) over the factor of the queries
-  // Value scales above it take the wide form of the loop: all, where heads have powers of their own.
-  float limit = kWide;
+  // Value scales above it take the wide form of the loop: all, where heads have powers of
+  // their own (-1) or a wait is to be given up (the check is in that copy alone: in both
+  // it cost 4 % of 1024 rows x 16 heads x 2048 tokens).
+  float limit = p.give_up ? -2.f : kWide;
   // Factors of this lane's tokens: of their scores, the exponent and the
   // inverse of their value scales (in the wide form, what makes their weights NaN).
   // True if one of them has a scale above the limit, or one that is NaN.
@@ -618,7 +624,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
       if (more && !again) prepare();
       again = false;
       // a wait that runs out ends the loop before the next copy
-      failed = !farq::mbar_wait_bounded(bars, parity, kAttnWaitNs);
+      failed = (WIDE && started == p.give_up) || !farq::mbar_wait_bounded(bars, parity, kAttnWaitNs);
       clear(kbox, mask);
 
       // scores of tiles of 16 tokens
@@ -763,7 +769,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
           pw[j][x] = transpose8x8(Half16<__half>::pack(w0, w1));
         }
 
-      failed = !farq::mbar_wait_bounded(bars + 8, parity, kAttnWaitNs);
+      failed = (WIDE && started == p.give_up) || !farq::mbar_wait_bounded(bars + 8, parity, kAttnWaitNs);
       clear(vbox, mask);
       // values times weights: rows g and g + 8 of output tile y are values 16y + g and 16y + g + 8
 #pragma unroll
@@ -797,15 +803,19 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
 #pragma unroll
     for (int x = 0; x < NB; ++x) {
       l[x] = mul2(l[x], pair(kSumUp, kSumUp));
-      if (limit == kWide && c == 0) reinterpret_cast<float*>(smem + L::ml)[warp * 2 * R + g + 8 * x] = 1.f;
+      if (limit != -1.f && c == 0) reinterpret_cast<float*>(smem + L::ml)[warp * 2 * R + g + 8 * x] = 1.f;
     }
     __syncwarp();
     work(std::true_type{});
   }
+  bool drained = true;
   if (__any_sync(0xffffffffu, failed)) {
-    // A copy did not arrive: wait (bounded) for those in flight, give NaN.
-    for (uint32_t i = started < 2 ? 0 : started - 2; i < started; ++i)
-      (void)farq::mbar_wait_bounded(bars + 8 * (i % 2), (i / 2) & 1, kAttnWaitNs);
+    // A copy did not arrive: wait (bounded) for those in flight, at most the last two
+    // of the two and more that were started; set the status and give NaN.
+    for (uint32_t i = started - 2; i < started; ++i)
+      drained &= farq::mbar_wait_bounded(bars + 8 * (i % 2), (i / 2) & 1, kAttnWaitNs);
+    drained = __all_sync(0xffffffffu, drained);
+    if (lane == 0 && p.status) atomicExch(p.status, (int)DSA_KV_ERR_DEVICE_TIMEOUT);
 #pragma unroll
     for (int x = 0; x < NB; ++x) l[x] = pair(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
   }
@@ -813,7 +823,8 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // Partial results into the warp's own ring, whose copies are all done.
+  // Partial results into the warp's own ring, whose copies are all done. Where one is
+  // still out after the second wait, the ring stays as it is: the join makes NaN of it.
   float* const ml = reinterpret_cast<float*>(smem + L::ml);
   float* const part = reinterpret_cast<float*>(smem + L::ring + (size_t)warp * L::region);
 #pragma unroll
@@ -828,6 +839,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
         ml[warp * 2 * R + row] = ref[x][e];
         ml[warp * 2 * R + R + row] = wide ? sum : sum * kSumUp;
       }
+      if (!drained) continue;
 #pragma unroll
       for (int y = 0; y < NT; ++y) {
         part[row * D + ((16 * y + g) ^ (c << 3))] = o[y][x][e];

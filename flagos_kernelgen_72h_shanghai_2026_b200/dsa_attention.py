@@ -32,7 +32,8 @@ def _selection(name, t, device, shape):
 def dsa_paged_attention(q: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Tensor,
                         v_cache: torch.Tensor, v_scale: torch.Tensor, blocks: torch.Tensor,
                         pages: torch.Tensor, q_pos: torch.Tensor, kv_lens: torch.Tensor,
-                        out: torch.Tensor, lse: torch.Tensor | None, softmax_scale: float):
+                        out: torch.Tensor, lse: torch.Tensor | None, softmax_scale: float, *,
+                        status: torch.Tensor | None = None, _test_copies: int = 0):
     """out = softmax(softmax_scale * q k^T) v over each row's selected tokens; returns ``(out, lse)``.
 
     q, out [B, Q, Hq, D] bf16 or fp16 (strided views whose rows start on 16
@@ -51,8 +52,12 @@ def dsa_paged_attention(q: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.T
     a value vector stored with a NaN or an infinity has out = NaN and the lse of
     its scores.
 
+    Waits of the kernel are bounded: a row whose copies have not arrived after
+    two seconds becomes NaN, and ``status``, an int32 tensor of one element if
+    given, 9 (it is never cleared).
+
     D is 64, 128 or 256; block_size is 8 to 65536."""
-    if L._fast is not None:
+    if L._fast is not None and status is None and not _test_copies:
         st = L._fast.kv_attn(q, k_cache, k_scale, v_cache, v_scale, blocks, pages, q_pos, kv_lens, out, lse,
                              softmax_scale)
         if st == 0:
@@ -97,11 +102,17 @@ def dsa_paged_attention(q: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.T
         if lse.dtype != torch.float32:
             raise TypeError(f"lse must be float32, got {lse.dtype}")
         a.lse = lse.data_ptr() or None
+    if status is not None:
+        L.check_tensor("status", status, dev)
+        L.check_shape("status", status, (1,))
+        if status.dtype != torch.int32:
+            raise TypeError(f"status must be int32, got {status.dtype}")
     a.softmax_scale = float(softmax_scale)
     a.B, a.Q, a.G, a.K = B, Q, Hq // H, K
     a.blocks = blocks.data_ptr() or None
     a.pages = pages.data_ptr() or None
     a.q_pos = q_pos.data_ptr() or None
     a.kv_lens = kv_lens.data_ptr() or None
-    L.launch(_OP, "dsa_kv_attn_launch", a, dev)
+    L.launch(_OP, "dsa_kv_attn_launch_status", a, dev,
+             status.data_ptr() if status is not None else None, _test_copies)
     return out, lse

@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define DSA_KV_ABI_VERSION 1
+#define DSA_KV_ABI_VERSION 2
 
 enum dsa_kv_dtype {
     DSA_KV_BF16 = 0,
@@ -51,7 +51,8 @@ enum dsa_kv_status {
     DSA_KV_ERR_ALIGNMENT = 5,     /* a pointer or a stride is not aligned          */
     DSA_KV_ERR_UNSUPPORTED = 6,   /* sizes beyond the kernel's index range         */
     DSA_KV_ERR_CUDA = 7,          /* a CUDA call failed                            */
-    DSA_KV_ERR_BAD_ARGS_SIZE = 8  /* struct_size mismatch or reserved field not 0  */
+    DSA_KV_ERR_BAD_ARGS_SIZE = 8, /* struct_size mismatch or reserved field not 0  */
+    DSA_KV_ERR_DEVICE_TIMEOUT = 9 /* a bounded device wait ran out                 */
 };
 
 /* A dense tensor [B, Q, H, D] whose last dimension is contiguous. Strides in
@@ -157,7 +158,7 @@ typedef struct dsa_kv_copy_args {
  * Products are fp16 x codes with sums in fp32: queries are scaled by a power of two,
  * bf16 values more than 2^-20 below their head's largest may lose bits.
  * out may be q itself. A copy that has not arrived after two seconds ends its
- * row: the outputs become NaN.
+ * row: the outputs become NaN, and dsa_kv_attn_launch_status says so.
  * v_scale is positive; one below 1e-12, the least that a write leaves, counts
  * as 1e-12. One that is NaN (a vector that held a NaN or an infinity) or infinite
  * makes out NaN in the rows that see its token; lse, which holds no values, is the
@@ -188,6 +189,15 @@ int dsa_kv_rope_launch(const dsa_kv_rope_args_t* args, void* stream);
 int dsa_kv_write_launch(const dsa_kv_copy_args_t* args, void* stream);
 int dsa_kv_read_launch(const dsa_kv_copy_args_t* args, void* stream);
 int dsa_kv_attn_launch(const dsa_kv_attn_args_t* args, void* stream);
+
+/*
+ * dsa_kv_attn_launch that tells a wait that ran out from NaN in the data: `status`,
+ * a device int or NULL, is then set to DSA_KV_ERR_DEVICE_TIMEOUT (it is never
+ * cleared). test_copies is 0, or, in tests of that path, a number of 2 and more:
+ * the first warp of every row that has started so many copies (keys and values of
+ * a chunk are one each) takes its next wait as run out, its copies in flight.
+ */
+int dsa_kv_attn_launch_status(const dsa_kv_attn_args_t* args, int32_t* status, int32_t test_copies, void* stream);
 
 /* Static string for a dsa_kv_status (never NULL). */
 const char* dsa_kv_strerror(int status);
