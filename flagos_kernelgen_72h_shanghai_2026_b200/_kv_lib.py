@@ -17,9 +17,9 @@ import torch
 from ._build import KV_LIB_PATH
 
 try:  # C++ launch path (csrc/farq_fast.cpp); without it every call takes the ctypes path
-    from . import _farq_fast as _fast
+    from . import _farq_fast as _extension
 except ImportError:
-    _fast = None
+    _extension = None
 
 # enum dsa_kv_dtype
 DTYPE_BF16, DTYPE_FP16, DTYPE_FP32, DTYPE_INT8, DTYPE_E4M3, DTYPE_INT32, DTYPE_INT64 = range(7)
@@ -37,6 +37,17 @@ ERR_BAD_ARGS_SIZE = 8
 ERR_DEVICE_TIMEOUT = 9
 
 ABI_VERSION = 2
+
+
+def launch_path(extension):
+    """The extension module, or None where it lacks this version's entry points: one built before they were
+    added, or next to a library of another version."""
+    if getattr(extension, "kv_abi_version", None) != ABI_VERSION:
+        return None
+    return extension if all(hasattr(extension, n) for n in ("kv_rope", "kv_copy", "kv_attn")) else None
+
+
+_fast = launch_path(_extension)
 
 HALF_DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_FP16}
 GAMMA_DTYPES = {**HALF_DTYPES, torch.float32: DTYPE_FP32}

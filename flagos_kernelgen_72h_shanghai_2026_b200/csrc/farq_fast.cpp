@@ -386,5 +386,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "C++ launch path of the Python operators";
   m.def("task01", &task01, "checks + farq_launch; status, or -1 when not handled");
   m.def("task02", &task02, "checks + dsa_topk_launch; status, or -1 when not handled");
-  if (PyModule_AddFunctions(m.ptr(), kKvMethods) != 0) throw py::error_already_set();
+  // Only for the library that these structs were laid out for: without the entry
+  // points every call takes the ctypes path, which refuses another version.
+  if (dsa_kv_abi_version() == DSA_KV_ABI_VERSION) {
+    m.attr("kv_abi_version") = DSA_KV_ABI_VERSION;
+    if (PyModule_AddFunctions(m.ptr(), kKvMethods) != 0) throw py::error_already_set();
+  }
 }

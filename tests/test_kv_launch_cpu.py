@@ -1,6 +1,7 @@
 """The launch paths of libdsa_kv.so without a GPU: the attention's entry with a
 status, and which C++ launch path is taken."""
 import ctypes
+from types import SimpleNamespace
 
 import pytest
 
@@ -27,3 +28,22 @@ def test_the_entry_with_a_status_validates_like_the_other(lib):
 
 def test_the_status_of_a_wait_has_a_name(lib):
     assert L.strerror(L.ERR_DEVICE_TIMEOUT) != L.strerror(99)
+
+
+def test_an_extension_without_the_entry_points_is_not_taken():
+    """One built before they were added has the other operators' alone; one of another version is no better."""
+    old = SimpleNamespace(task01=print, task02=print)
+    kv = dict(kv_rope=print, kv_copy=print, kv_attn=print)
+    assert L.launch_path(None) is None and L.launch_path(old) is None
+    assert L.launch_path(SimpleNamespace(**kv)) is None
+    assert L.launch_path(SimpleNamespace(kv_abi_version=L.ABI_VERSION - 1, **kv)) is None
+    assert L.launch_path(SimpleNamespace(kv_abi_version=L.ABI_VERSION, kv_rope=print, kv_copy=print)) is None
+    now = SimpleNamespace(kv_abi_version=L.ABI_VERSION, **kv)
+    assert L.launch_path(now) is now
+
+
+def test_the_built_extension_is_taken():
+    from flagos_kernelgen_72h_shanghai_2026_b200._build import build_fast_ext
+    build_fast_ext()
+    from flagos_kernelgen_72h_shanghai_2026_b200 import _farq_fast
+    assert L.launch_path(_farq_fast) is _farq_fast and L._fast is _farq_fast
