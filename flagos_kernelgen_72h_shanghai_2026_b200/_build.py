@@ -105,7 +105,11 @@ def fast_ext_path() -> Path:
 def build_fast_ext(force: bool = False, verbose: bool = False) -> Path:
     """Compile the C++ launch path of the Python operators (_farq_fast, a
     torch extension module linked against libfarq.so, libdsa_topk.so and
-    libdsa_kv.so) with g++, in-tree, if it is missing or older than its sources."""
+    libdsa_kv.so) with g++, in-tree, if it is missing or older than its sources.
+    A library that is not there yet is built first."""
+    for path, build in ((LIB_PATH, build_lib), (TOPK_LIB_PATH, build_topk_lib), (KV_LIB_PATH, build_kv_lib)):
+        if not path.exists():
+            build(verbose=verbose)
     out = fast_ext_path()
     deps = [FAST_SOURCE, INCLUDE_DIR / "farq.h", INCLUDE_DIR / "dsa_topk.h",
             INCLUDE_DIR / "dsa_kv.h", LIB_PATH, TOPK_LIB_PATH, KV_LIB_PATH]

@@ -1,6 +1,7 @@
 """The launch paths of libdsa_kv.so without a GPU: the attention's entry with a
 status, and which C++ launch path is taken."""
 import ctypes
+import os
 from types import SimpleNamespace
 
 import pytest
@@ -47,3 +48,25 @@ def test_the_built_extension_is_taken():
     build_fast_ext()
     from flagos_kernelgen_72h_shanghai_2026_b200 import _farq_fast
     assert L.launch_path(_farq_fast) is _farq_fast and L._fast is _farq_fast
+
+
+def test_the_extension_builds_where_a_library_is_not_there_yet(monkeypatch, tmp_path):
+    """A tree built before libdsa_kv.so was added: the library is built, then linked."""
+    from flagos_kernelgen_72h_shanghai_2026_b200 import _build as B
+    lib, out, done = tmp_path / "libdsa_kv.so", tmp_path / "_farq_fast.so", []
+    out.write_bytes(b"before")
+    os.utime(out, (0, 0))
+
+    def build(verbose=False):
+        done.append("library")
+        lib.write_bytes(b"")
+
+    def run(cmd, verbose):
+        done.append("link")
+        (tmp_path / "_farq_fast.so.tmp").write_bytes(b"after")
+        return ""
+
+    for name, v in (("KV_LIB_PATH", lib), ("build_kv_lib", build), ("_run", run), ("fast_ext_path", lambda: out)):
+        monkeypatch.setattr(B, name, v)
+    assert B.build_fast_ext() == out
+    assert done == ["library", "link"] and out.read_bytes() == b"after"
