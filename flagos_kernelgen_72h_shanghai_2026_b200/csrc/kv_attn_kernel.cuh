@@ -836,7 +836,8 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
       for (int y = 4; y <= 16; y <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, y);
       const int row = 2 * c + e + 8 * x;
       if (g == 0) {
-        ml[warp * 2 * R + row] = ref[x][e];
+        // Tokens whose scores are all -inf are not the same as none.
+        ml[warp * 2 * R + row] = ref[x][e] == -INFINITY && (started << 2) != 0 ? -3.4028235e38f : ref[x][e];
         ml[warp * 2 * R + R + row] = wide ? sum : sum * kSumUp;
       }
       if (!drained) continue;
@@ -853,7 +854,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     const float h = exp2_approx(0.5f * d);
     return d < kTwoSteps ? fmaf(h * l, h, total) : fmaf(w, l, total);
   };
-  auto finish = [&](float total) { return total == 0.f ? 0.f : 1.0f / total; };
+  auto finish = [&](float m, float total) { return m == -INFINITY && total == 0.f ? 0.f : 1.0f / total; };
   auto put_lse = [&](int row, float m, float total) {
     p.lse[((int64_t)b * p.Q.d + qi) * p.H.d * p.G + head0 + row] =
         total == 0.f ? -INFINITY : (m + log2f(total)) * 0.69314718055994531f;
@@ -884,7 +885,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
       total = add_sum(total, ml[n * 2 * R + R + row], w[n], d);
     }
     total *= 1.f / kSumUp;
-    const float f = finish(total);
+    const float f = finish(m, total);
 #pragma unroll
     for (int k = 0; k < D / 4 / LPR; ++k) {
       const int f4 = sub + k * LPR, at = part_index<D>(row, f4);
@@ -963,7 +964,7 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
     for (int y = 1; y < LPR; y <<= 1) total += __shfl_xor_sync(0xffffffffu, total, y);
     total *= 1.f / kSumUp;
     if (sub == 0) {
-      fin[row] = finish(total);
+      fin[row] = finish(m, total);
       if (p.lse && rank == 0 && row < rows) put_lse(row, m, total);
     }
   }

@@ -155,6 +155,7 @@ typedef struct dsa_kv_copy_args {
  * counts twice.
  *     out = sum_t softmax(scale * q.k_t) v_t,   lse = ln sum_t exp(scale * q.k_t)
  * A row without a token (and a padded one, q_pos < 0) has out = 0, lse = -inf.
+ * One whose tokens all have the score -inf has out = NaN, lse = -inf.
  * Products are fp16 x codes with sums in fp32: queries are scaled by a power of two,
  * bf16 values more than 2^-20 below their head's largest may lose bits.
  * out may be q itself. A copy that has not arrived after two seconds ends its

@@ -157,6 +157,27 @@ def test_scores_a_few_places_apart(dev, e, above):
         assert abs(out.float() - want).max() <= want * (2.0 ** -8 + 2.0 ** -18) + 512 * 2.0 ** -20, (delta, want)
 
 
+@pytest.mark.parametrize("B,Q,K,G,D,bs", SHAPES, ids=str)
+def test_scores_of_minus_infinity(dev, B, Q, K, G, D, bs):
+    """A query of -inf on keys that are all positive there: tokens, but no finite score. out is NaN and not the zeros of
+    a row without tokens, lse is -inf for both; where some tokens have the code 0 there, the score is NaN."""
+    _, _, _, c, q, blocks, pages, pos, lens = inputs(85 + G, B=B, Q=Q, G=G, D=D, bs=bs, K=K, NB=K + 1, code=INT8)
+    c[0][..., 3] = c[0][..., 3].abs().clamp(min=1)
+    c[0][c[1].argmax() % c[0].shape[0], :, 0, 3] = 0
+    q[..., 0, 3] = -math.inf
+    if Q > 1:
+        pos[0, 1] = -1
+    r = R.dsa_paged_attention_ref(q, *c, blocks, pages, pos, lens, 0.1)
+    out, lse = run(dev, q, c, blocks, pages, pos, lens, 0.1)
+    seen = (pos >= 0)[..., None].expand(r["lse"].shape)
+    first = torch.arange(2 * G) == 0
+    assert torch.equal(out.cpu().isnan(), r["out"].isnan())
+    assert out.cpu()[seen & first].isnan().all() and (out.cpu()[~seen] == 0).all()
+    assert torch.equal(lse.cpu() == -math.inf, r["lse"] == -math.inf)
+    ok = {k: v[~first.expand(r["lse"].shape)] for k, v in r.items()}
+    check(out.cpu()[~first.expand(r["lse"].shape)], lse.cpu()[~first.expand(r["lse"].shape)], ok, D, 127.0)
+
+
 # ------------------------------------------------------- heads of unlike size
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("code", [E4M3, INT8])
