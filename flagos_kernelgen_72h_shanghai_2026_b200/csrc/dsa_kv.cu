@@ -79,8 +79,10 @@ int rope(const dsa_kv_rope_args_t* a, void* stream) {
   if (!bind_device(&dev) || !sm_count(dev, &sms)) return DSA_KV_ERR_CUDA;
   // Steps of two heads to a group of lanes where each then has a warp to itself on
   // one CTA per SM, else of four. Device time in us with two / four, 40 heads x
-  // 128: 1 token 2.16 / 2.47, 32 tokens 2.37 / 2.77, 96 tokens 2.46 / 2.87, 128
-  // tokens (160 CTAs) 2.98 / 2.88, 384 tokens 3.90 / 3.49, 8192 tokens 49 / 33.4.
+  // 128: 1 token 2.06 / 2.47, 32 tokens 2.47 / 2.77, 96 tokens 2.47 / 2.87, 128
+  // tokens (160 CTAs) 2.98 / 2.88, 384 tokens 3.92 / 3.49, 8192 tokens 49 / 33.4 to 34.4.
+  // Places of a step that heads leave empty are not looked at: 24 + 4 heads of 64 fill 28
+  // of 48 with four (1665 tokens 5.3 us either way).
   const int lanes = lanes_of(a->D);
   int u = 2;
   int64_t steps_q, per_token;
@@ -155,8 +157,8 @@ int copy(const dsa_kv_copy_args_t* a, void* stream, bool write) {
   while ((1 << (log_hps + log_tpw)) < groups) ++log_tpw;
   const int64_t steps = ceil_div(c.H, 1 << log_hps);
   // Steps per lane, as many as there are up to 4. At 8 heads x 128 (us with
-  // 1 / 2 / 4): write of 2 x 4096 tokens 12.8 / 11.0 / 10.9, read of 8 x up to
-  // 8192 tokens 63.2 / 56.4 / 53.8; calls of 64 and of 333 tokens do not care.
+  // 1 / 2 / 4): write of 2 x 4096 tokens 13.0 / 11.0 / 11.0, read of 8 x up to
+  // 8192 tokens 71.1 / 53.7 / 51.9; calls of 64 and of 333 tokens do not care.
   const int u = steps >= 4 ? 4 : steps >= 2 ? 2 : 1;
   const int64_t strips = ceil_div(steps, u), tokens = a->B * a->Q;
   p.tasks = (uint32_t)(ceil_div(tokens, 1 << log_tpw) * strips);

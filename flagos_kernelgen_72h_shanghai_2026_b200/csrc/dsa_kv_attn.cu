@@ -142,9 +142,10 @@ int attn(const dsa_kv_attn_args_t* a, int32_t* status, int32_t test_copies, void
   // 8 CTAs, 4 query heads, D = 128): 8 tiles of 8 chunks 6.3 / 6.8 / 7.3 / 7.3, of
   // 16 chunks 9.2 / 8.3 / 7.3 / 7.5, of 32 chunks 14.9 / 11.2 / 8.7 / 7.7; 64 tiles
   // of 32 chunks 16.0 / 12.4 / 11.4 / 18.5; 144 tiles of 16 chunks 12.2 / 13.0 /
-  // 19.4 / 30.9. Over 738 cases of every head size the choice is 1.6 % off the best
-  // in the mean and 24 % at worst; as many CTAs as the SMs hold were 5.6 %, and up
-  // to 82 % where clusters did not fit the groups of SMs that hold one together.
+  // 19.4 / 30.9. Over 738 cases of every head size the choice is 1.4 % off the best
+  // in the mean and 29 % at worst (profiles/dsa_paged_attention_clusters.md); as many
+  // CTAs as the SMs hold were 5.6 %, and up to 82 % where clusters did not fit the
+  // groups of SMs that hold one together.
   int log_c = 0, per_sm = tiles <= (int64_t)sms * v.ctas ? (int)ceil_div(tiles, sms) : v.ctas;
   {
     const int join2[4] = {0, 3, 4, 5};  // twice the rounds of a join

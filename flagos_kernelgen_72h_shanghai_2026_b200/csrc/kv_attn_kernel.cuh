@@ -55,14 +55,22 @@
 // weights change sides with movmatrix.
 //
 // Why mma.sync: a row has at most 16 heads to multiply a key with, the least
-// tile of tcgen05 has 64 or 128 rows; with tokens as those rows the codes would
-// have to be written back to shared memory as fp16 first.
+// tile of tcgen05 has 64 or 128 rows; with tokens as those rows fp16 operands would
+// mean to write the codes back to shared memory widened. Its 8-bit kinds take the
+// codes as they are copied, with queries and weights cut into 8-bit terms; that form
+// has not been built.
 //
 // What bounds it: a decode batch is bound by HBM (32 rows x 8 key heads over 8192
-// e4m3 tokens of D = 128: 87 us, 6.4 TB/s). Rows whose pages stay in L2 are bound
-// by what the warps issue: 265 cycles per SM for 32 tokens of 16 heads at
-// D = 128 (1024 rows x 2048 tokens: 85.5 us), of which the tensor pipe needs 128
-// and the conversion of codes, on the half-rate integer pipe, 64.
+// e4m3 tokens of D = 128: 87.4 us, 6.35 TB/s). Rows whose pages stay in L2 are bound
+// by latency at 8 warps per SM (1024 rows x 16 heads x 2048 tokens, D = 128: 86.7 us):
+// issue slots are 37 % and the tensor pipe 37 % busy; a chunk is a chain of wait, scores,
+// maximum, exponentials, weights turned around, outputs, and 254 registers hold
+// two CTAs. 32 tokens of 16 heads take an SM 385 cycles there at 1965 MHz in the mean, 274
+// as the slope from 64 to 128 blocks; the tensor pipe needs 128 of them, the
+// conversion of codes, on the half-rate integer pipe, 64. The mean holds the rows' start
+// and join and the last wave: 1024 CTAs on 296 places are 3.46 waves, worth 13 %.
+// The second copy of the loop (value scales above 2^32 or not finite, heads of
+// unlike size) takes 23 % longer for values of that kind there, 7 % for such heads.
 #pragma once
 
 #include <cuda.h>
@@ -913,8 +921,9 @@ __global__ void __launch_bounds__(kAttnThreads, CTAS)
   float* const all = reinterpret_cast<float*>(smem + L::all);
   float* const fin = reinterpret_cast<float*>(smem + L::fin);
   // Four values go to 2^log_lanes lanes. Where a lane has few partial results,
-  // they are on their way while the weights are worked out (one row of 4 heads
-  // over 2048 tokens, D = 128: 7.0 instead of 7.6 us).
+  // they are on their way while the weights are worked out (8 rows of 4 heads over
+  // 2048 tokens, D = 128: 7.0 instead of 7.6 us; where several clusters share an SM it
+  // costs more than it hides, 32 rows over 4096 tokens 12.6 instead of 12.1 us).
   constexpr int AHEAD = 8;
   const int units = rows * (D / 4), share = (units + (int)C - 1) >> (__ffs(C) - 1);
   int log_lanes = 0;

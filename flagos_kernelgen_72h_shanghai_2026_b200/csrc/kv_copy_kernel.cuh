@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(kCopyThreads) write_kernel(const CopyParams p)
   float inv = __frcp_rn(scale);
   if (mine >= Half16<T>::kInf) {
     scale = __int_as_float(0x7fc00000);
-    inv = 0.f;  // marks codes 0 (no finite vector has it: scale is below 1e36)
+    inv = 0.f;  // marks codes 0 (no finite vector has it: 3.39e38 / 127 < 2.7e36, whose inverse is a normal number)
   }
   if (cell && i < NV && w.h + (i % U) * hps < p.H) {
     const CacheSide& c = i < U ? p.kc : p.vc;

@@ -152,7 +152,7 @@ typedef struct dsa_kv_copy_args {
  *     t <= q_pos[b, q],  t < kv_lens[b]
  * whose keys and values lie in page pages[i]. An entry with a negative block
  * id, or a page id outside [0, P), stands for none; one that occurs twice
- * counts twice.
+ * counts twice. No token lies at position 2^40 or beyond.
  *     out = sum_t softmax(scale * q.k_t) v_t,   lse = ln sum_t exp(scale * q.k_t)
  * A row without a token (and a padded one, q_pos < 0) has out = 0, lse = -inf.
  * One whose tokens all have the score -inf has out = NaN, lse = -inf.
