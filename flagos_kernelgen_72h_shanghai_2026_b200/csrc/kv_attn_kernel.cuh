@@ -61,16 +61,16 @@
 // has not been built.
 //
 // What bounds it: a decode batch is bound by HBM (32 rows x 8 key heads over 8192
-// e4m3 tokens of D = 128: 87.4 us, 6.35 TB/s). Rows whose pages stay in L2 are bound
-// by latency at 8 warps per SM (1024 rows x 16 heads x 2048 tokens, D = 128: 86.7 us):
+// e4m3 tokens of D = 128: 87 to 88 us, 6.3 TB/s). Rows whose pages stay in L2 are bound
+// by latency at 8 warps per SM (1024 rows x 16 heads x 2048 tokens, D = 128: 85.4 us):
 // issue slots are 37 % and the tensor pipe 37 % busy; a chunk is a chain of wait, scores,
 // maximum, exponentials, weights turned around, outputs, and 254 registers hold
-// two CTAs. 32 tokens of 16 heads take an SM 385 cycles there at 1965 MHz in the mean, 274
+// two CTAs. 32 tokens of 16 heads take an SM 379 cycles there at 1965 MHz in the mean, 274
 // as the slope from 64 to 128 blocks; the tensor pipe needs 128 of them, the
 // conversion of codes, on the half-rate integer pipe, 64. The mean holds the rows' start
 // and join and the last wave: 1024 CTAs on 296 places are 3.46 waves, worth 13 %.
 // The second copy of the loop (value scales above 2^32 or not finite, heads of
-// unlike size) takes 23 % longer for values of that kind there, 7 % for such heads.
+// unlike size) takes 24 % longer for values of that kind there, 8 % for such heads.
 #pragma once
 
 #include <cuda.h>
