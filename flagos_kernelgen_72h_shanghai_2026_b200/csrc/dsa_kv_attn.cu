@@ -143,7 +143,7 @@ int attn(const dsa_kv_attn_args_t* a, int32_t* status, int32_t test_copies, void
   // 16 chunks 9.2 / 8.3 / 7.3 / 7.5, of 32 chunks 14.9 / 11.2 / 8.7 / 7.7; 64 tiles
   // of 32 chunks 16.0 / 12.4 / 11.4 / 18.5; 144 tiles of 16 chunks 12.2 / 13.0 /
   // 19.4 / 30.9. Over 738 cases of every head size the choice is 1.4 % off the best
-  // in the mean and 29 % at worst (profiles/dsa_paged_attention_clusters.md); as many
+  // in the mean and 29 % at worst (32 to 48 tiles of 32 blocks, 8 CTAs for 4); as many
   // CTAs as the SMs hold were 5.6 %, and up to 82 % where clusters did not fit the
   // groups of SMs that hold one together.
   int log_c = 0, per_sm = tiles <= (int64_t)sms * v.ctas ? (int)ceil_div(tiles, sms) : v.ctas;
